@@ -19,7 +19,7 @@ from .export import (
     unpack_u4_indices,
 )
 from .calibration import ActivationRangeCollector, apply_activation_qparams, calibrate_activation_qparams
-from .modules import DIMQConv2d, DIMQLinear, make_packed_layer, replace_modules_with_packed_dimq
+from .modules import DIMQConv2d, DIMQLinear, MXLinear, make_packed_layer, replace_modules_with_packed_dimq
 from .ops import (
     build_product_table,
     dimq_conv2d_lut,
@@ -28,6 +28,11 @@ from .ops import (
     dimq_linear_wq,
     hard_quantize,
     is_available,
+    mx_dequantize,
+    mx_linear,
+    mx_linear_grad_input,
+    mx_linear_grad_weight,
+    mx_quantize,
     pack_bits,
     pack_u4,
     quantize_activation_u4,
@@ -37,11 +42,12 @@ from .ops import (
 )
 
 __all__ = [
-    "ActivationRangeCollector", "DIMQConv2d", "DIMQLinear", "activation_qparams_from_minmax", "apply_activation_qparams",
+    "ActivationRangeCollector", "DIMQConv2d", "DIMQLinear", "MXLinear", "activation_qparams_from_minmax", "apply_activation_qparams",
     "calibrate_activation_qparams", "assign_weight_indices", "build_product_table",
     "default_activation_qparams", "dimq_conv2d_lut", "dimq_conv2d_wq", "dimq_linear_lut", "dimq_linear_wq",
     "export_compact_checkpoint", "export_packed_dimq_checkpoint", "hard_quantize", "hard_quantize_weight",
-    "infer_module_hparams", "is_available", "load_compact_checkpoint", "make_packed_layer", "pack_bits", "pack_u4",
+    "infer_module_hparams", "is_available", "load_compact_checkpoint", "make_packed_layer",
+    "mx_dequantize", "mx_linear", "mx_linear_grad_input", "mx_linear_grad_weight", "mx_quantize", "pack_bits", "pack_u4",
     "pack_u4_indices", "quantize_activation_u4", "replace_modules_with_packed_dimq", "require_extension",
     "unpack_bits", "unpack_u4", "unpack_u4_indices",
 ]

@@ -725,6 +725,239 @@ Tensor attention_qkv(const Tensor& qkv, int64_t heads, int* launches) {
   return y;
 }
 
+// ---- microscaled numbers ----------------------------------------------------------------------------
+
+struct MxSizes {
+  int64_t pitch, scale_bytes, row_tiles, block_tiles;
+};
+
+MxSizes mx_sizes(int64_t rows, int64_t cols, int format) {
+  MxSizes s;
+  check(dimq_mx_sizes(rows, cols, format, &s.pitch, &s.scale_bytes), "mx_sizes");
+  s.row_tiles = (rows + 127) / 128;
+  s.block_tiles = (cols + 127) / 128;
+  return s;
+}
+
+at::ScalarType mx_code_type(int format) { return format == DIMQ_MX_FP4 ? at::kByte : at::kChar; }
+
+Tensor aligned16(const Tensor& t) {   // the kernels' 16-byte loads and tensor maps
+  Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+struct Mx {   // codes and scales of a matrix, empty
+  Tensor codes, scales;
+};
+
+Mx mx_empty(at::IntArrayRef lead, int64_t rows, int64_t cols, int format, const Tensor& like) {
+  const MxSizes s = mx_sizes(rows, cols, format);
+  std::vector<int64_t> shape(lead.begin(), lead.end());
+  shape.push_back(s.pitch);
+  const auto opt = like.options().memory_format(at::MemoryFormat::Contiguous);
+  return {at::empty(shape, opt.dtype(mx_code_type(format))), at::empty({s.row_tiles, s.block_tiles, 512}, opt.dtype(at::kByte))};
+}
+
+// codes [..., pitch] and scales of `rows` rows (-1: as many as the codes have) of `cols` values
+Mx mx_operand(const Tensor& codes, const Tensor& scales, int64_t* rows, int64_t cols, int format, const char* what) {
+  const std::string name(what);
+  if (!codes.is_cuda() || !scales.is_cuda()) fail(name + " codes and scales must be CUDA tensors");
+  same_device(scales, codes, (name + " scales").c_str());
+  if (codes.scalar_type() != mx_code_type(format))
+    fail(name + " codes must be " + (format == DIMQ_MX_FP4 ? "uint8" : "int8") + ", got " + c10::toString(codes.scalar_type()));
+  if (scales.scalar_type() != at::kByte) fail(name + std::string(" scales must be uint8, got ") + c10::toString(scales.scalar_type()));
+  const MxSizes one = mx_sizes(1, cols, format);
+  if (codes.dim() == 0 || codes.size(-1) != one.pitch)
+    fail(name + " codes must have a last dimension of " + std::to_string(one.pitch) + " for " + std::to_string(cols) + " values");
+  const int64_t have = codes.numel() / one.pitch;
+  if (*rows >= 0 && have != *rows) fail(name + " codes must have " + std::to_string(*rows) + " rows, got " + std::to_string(have));
+  *rows = have;
+  const MxSizes s = mx_sizes(have, cols, format);
+  if (scales.numel() != s.scale_bytes)
+    fail(name + " scales must be [" + std::to_string(s.row_tiles) + ", " + std::to_string(s.block_tiles) + ", 512]");
+  return {aligned16(codes), aligned16(scales)};
+}
+
+int mx_format(int64_t f) {
+  if (f != DIMQ_MX_FP4 && f != DIMQ_MX_INT8) fail("unknown microscaled format " + std::to_string(f));
+  return static_cast<int>(f);
+}
+
+int64_t mx_rows(const Tensor& x, int64_t cols) { return x.numel() / cols; }
+
+Mx mx_quantize(const Tensor& x, int format, int* launches) {
+  require_cuda(x, "mx_quantize");
+  const int xd = dtype_code(x, "x");
+  if (x.dim() == 0 || x.size(-1) <= 0) fail("mx_quantize expects a last dimension of at least one value");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor xc = x.contiguous();
+  const int64_t cols = x.size(-1), rows = mx_rows(x, cols);
+  Mx q = mx_empty(x.sizes().slice(0, x.dim() - 1), rows, cols, format, x);
+  check(dimq_mx_quantize(xc.data_ptr(), xd, rows, cols, format, q.codes.data_ptr(), static_cast<uint8_t*>(q.scales.data_ptr()),
+                         stream_of(x)), "mx_quantize");
+  *launches = rows > 0;
+  return q;
+}
+
+const uint8_t* bytes_of(const Tensor& t) { return static_cast<const uint8_t*>(t.data_ptr()); }
+uint8_t* writable(Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+Tensor mx_dequantize(const Tensor& codes, const Tensor& scales, int64_t cols, int format, at::ScalarType dt, int* launches) {
+  int64_t rows = -1;
+  if (cols <= 0) fail("mx_dequantize expects at least one feature");
+  const c10::cuda::OptionalCUDAGuard guard(codes.is_cuda() ? std::optional<c10::Device>(codes.device()) : std::nullopt);
+  const Mx q = mx_operand(codes, scales, &rows, cols, format, "mx_dequantize");
+  Tensor y = at::empty(out_shape(codes, cols), codes.options().dtype(dt).memory_format(at::MemoryFormat::Contiguous));
+  check(dimq_mx_dequantize(q.codes.data_ptr(), bytes_of(q.scales), format, rows, cols, y.data_ptr(), dtype_code(y, "out_dtype"),
+                           stream_of(codes)), "mx_dequantize");
+  *launches = rows > 0;
+  return y;
+}
+
+// x: values, or (x_scales) the codes of a 4-bit quantisation
+void mx_linear_into(const Tensor& x, int xd, const OptTensor& x_scales, const Mx& w, const Bias& b, const OptTensor& res, Tensor& y,
+                    int64_t m, int64_t n, int64_t k, int epilogue, int* launches) {
+  int64_t need = 0;
+  check(dimq_mx_linear_workspace_bytes(m, n, k, x_scales.has_value(), &need), "mx_linear_workspace_bytes");
+  OptTensor ws;
+  if (need > 0 && m > 0) ws = scratch(need, x);
+  check(dimq_mx_linear(x.data_ptr(), xd, x_scales.has_value() ? bytes_of(*x_scales) : nullptr, bytes_of(w.codes), bytes_of(w.scales),
+                       ptr(b.t), b.dtype, ptr(res), y.data_ptr(), dtype_code(y, "y"), m, n, k, epilogue,
+                       ws.has_value() ? ws->data_ptr() : nullptr, need, stream_of(x)), "mx_linear");
+  *launches += m > 0 ? 1 + (need > 0) : 0;
+}
+
+Tensor mx_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& bias, int64_t n, int64_t k,
+                 at::ScalarType out_dtype, int epilogue, const OptTensor& residual, int* launches) {
+  require_cuda(x, "mx_linear");
+  const int xd = dtype_code(x, "x");
+  if (n <= 0 || k <= 0) fail("linear dimensions must be positive");
+  if (x.dim() == 0 || x.size(-1) != k) fail("input last dimension must equal in_features");
+  same_device(codes, x, "weight codes");
+  const c10::cuda::CUDAGuard guard(x.device());
+  int64_t rows = n;
+  const Mx w = mx_operand(codes, scales, &rows, k, DIMQ_MX_FP4, "weight");
+  const Bias b = bias_arg(bias, x, n, "out_features");
+  const Tensor xc = x.contiguous();
+  Tensor y = at::empty(out_shape(x, n), x.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
+  const OptTensor res = linear_residual(residual, y);
+  mx_linear_into(xc, xd, std::nullopt, w, b, res, y, mx_rows(x, k), n, k, epilogue, launches);
+  return y;
+}
+
+// The layer's forward for training: y, what its backward needs of x (keep: 0 nothing, else the format) and of w.
+struct MxForward {
+  Tensor y;
+  OptTensor x_codes, x_scales;
+  Mx w;
+};
+
+MxForward mx_layer_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, int keep, int* launches) {
+  require_cuda(x, "mx_linear");
+  require_cuda(weight, "mx_linear");
+  same_device(weight, x, "weight");
+  const int xd = dtype_code(x, "x"), wd = dtype_code(weight, "weight");
+  if (weight.dim() != 2 || weight.size(0) <= 0 || weight.size(1) <= 0) fail("weight must be [out_features, in_features]");
+  const int64_t n = weight.size(0), k = weight.size(1);
+  if (x.dim() == 0 || x.size(-1) != k) fail("input last dimension must equal in_features");
+  const Bias b = bias_arg(bias, x, n, "out_features");
+  const c10::cuda::CUDAGuard guard(x.device());
+  void* st = stream_of(x);
+  const Tensor xc = x.contiguous(), wc = weight.contiguous();
+  const int64_t m = mx_rows(x, k);
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  MxForward f;
+  f.w = mx_empty({n}, n, k, DIMQ_MX_FP4, x);
+  check(dimq_mx_quantize(wc.data_ptr(), wd, n, k, DIMQ_MX_FP4, f.w.codes.data_ptr(), writable(f.w.scales), st), "mx_quantize");
+  Mx x4 = mx_empty(lead, m, k, DIMQ_MX_FP4, x);
+  if (keep == DIMQ_MX_INT8) {
+    Mx x8 = mx_empty(lead, m, k, DIMQ_MX_INT8, x);
+    check(dimq_mx_quantize_both(xc.data_ptr(), xd, m, k, writable(x4.codes), writable(x4.scales),
+                                static_cast<int8_t*>(x8.codes.data_ptr()), writable(x8.scales), st), "mx_quantize_both");
+    f.x_codes = x8.codes;
+    f.x_scales = x8.scales;
+  } else {
+    check(dimq_mx_quantize(xc.data_ptr(), xd, m, k, DIMQ_MX_FP4, x4.codes.data_ptr(), writable(x4.scales), st), "mx_quantize");
+    if (keep == DIMQ_MX_FP4) {
+      f.x_codes = x4.codes;
+      f.x_scales = x4.scales;
+    }
+  }
+  *launches += 1 + (m > 0);
+  f.y = at::empty(out_shape(x, n), x.options().memory_format(at::MemoryFormat::Contiguous));
+  mx_linear_into(x4.codes, 0, x4.scales, f.w, b, std::nullopt, f.y, m, n, k, DIMQ_EPI_NONE, launches);
+  return f;
+}
+
+Tensor mx_grad_scratch(const Tensor& dy, int dyd, int64_t m, int64_t n, int64_t k, int64_t* need) {
+  check(dimq_mx_grad_workspace_bytes(dyd, m, n, k, need), "mx_grad_workspace_bytes");
+  return scratch(*need, dy);
+}
+
+Tensor mx_grad_input(const Tensor& dy, const Tensor& codes, const Tensor& scales, int64_t k, at::ScalarType dt, int* launches) {
+  require_cuda(dy, "mx_linear_grad_input");
+  const int dyd = dtype_code(dy, "grad");
+  if (dy.dim() == 0 || dy.size(-1) <= 0) fail("mx_linear_grad_input expects a last dimension of out_features");
+  if (k <= 0) fail("linear dimensions must be positive");
+  same_device(codes, dy, "weight codes");
+  const c10::cuda::CUDAGuard guard(dy.device());
+  int64_t n = dy.size(-1);
+  const Mx w = mx_operand(codes, scales, &n, k, DIMQ_MX_FP4, "weight");
+  const Tensor g = dy.contiguous();
+  Tensor dx = at::empty(out_shape(dy, k), dy.options().dtype(dt).memory_format(at::MemoryFormat::Contiguous));
+  const int64_t m = mx_rows(dy, n);
+  int64_t need = 0;
+  const Tensor ws = mx_grad_scratch(g, dyd, m, n, k, &need);
+  check(dimq_mx_grad_input(g.data_ptr(), dyd, bytes_of(w.codes), bytes_of(w.scales), dx.data_ptr(), dtype_code(dx, "out_dtype"), m, n,
+                           k, ws.data_ptr(), need, stream_of(dy)), "mx_linear_grad_input");
+  *launches += m > 0 ? 2 : 0;
+  return dx;
+}
+
+// (dw, db): dw where dw_dtype, db where db_dtype is given
+std::pair<OptTensor, OptTensor> mx_grad_weight(const Tensor& dy, const Tensor& codes, const Tensor& scales, int64_t k, int format,
+                                               std::optional<at::ScalarType> dw_dtype, std::optional<at::ScalarType> db_dtype,
+                                               int* launches) {
+  require_cuda(dy, "mx_linear_grad_weight");
+  const int dyd = dtype_code(dy, "grad");
+  if (dy.dim() == 0 || dy.size(-1) <= 0) fail("mx_linear_grad_weight expects a last dimension of out_features");
+  if (k <= 0) fail("linear dimensions must be positive");
+  const c10::cuda::CUDAGuard guard(dy.device());
+  const int64_t n = dy.size(-1);
+  int64_t m = mx_rows(dy, n);
+  same_device(codes, dy, "activation codes");
+  const Mx x = mx_operand(codes, scales, &m, k, format, "activation");
+  const Tensor g = dy.contiguous();
+  OptTensor dw, db;
+  const auto opt = dy.options().memory_format(at::MemoryFormat::Contiguous);
+  if (dw_dtype.has_value()) dw = at::empty({n, k}, opt.dtype(*dw_dtype));
+  if (db_dtype.has_value()) db = at::empty({n}, opt.dtype(*db_dtype));
+  int64_t need = 0;
+  const Tensor ws = mx_grad_scratch(g, dyd, m, n, k, &need);
+  check(dimq_mx_grad_weight(g.data_ptr(), dyd, x.codes.data_ptr(), bytes_of(x.scales), format, dw.has_value() ? dw->data_ptr() : nullptr,
+                            dw.has_value() ? dtype_code(*dw, "out_dtype") : 0, db.has_value() ? db->data_ptr() : nullptr,
+                            db.has_value() ? dtype_code(*db, "bias dtype") : 0, m, n, k, ws.data_ptr(), need, stream_of(dy)),
+        "mx_linear_grad_weight");
+  *launches += (dw.has_value() ? 2 : 0) + (db.has_value() ? 1 : 0);
+  return {dw, db};
+}
+
+Tensor mx_column_sum(const Tensor& dy, at::ScalarType dt, int* launches) {
+  require_cuda(dy, "mx_column_sum");
+  const int dyd = dtype_code(dy, "grad");
+  if (dy.dim() == 0 || dy.size(-1) <= 0) fail("mx_column_sum expects a last dimension of out_features");
+  const c10::cuda::CUDAGuard guard(dy.device());
+  const Tensor g = dy.contiguous();
+  const int64_t n = dy.size(-1), m = mx_rows(dy, n);
+  Tensor db = at::empty({n}, dy.options().dtype(dt).memory_format(at::MemoryFormat::Contiguous));
+  int64_t need = 0;
+  const Tensor ws = mx_grad_scratch(g, dyd, m, n, 1, &need);
+  check(dimq_mx_grad_weight(g.data_ptr(), dyd, nullptr, nullptr, DIMQ_MX_INT8, nullptr, 0, db.data_ptr(), dtype_code(db, "bias dtype"),
+                            m, n, 1, ws.data_ptr(), need, stream_of(dy)), "mx_linear_grad_weight");
+  *launches += 1;
+  return db;
+}
+
 // ---- the Python module ----------------------------------------------------------------------------
 
 #define ARGS(want, name) want_args(n, want, name)
@@ -933,6 +1166,120 @@ PyObject* py_images_to_nhwc(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_mx_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  ARGS(2, "mx_quantize");
+  const Tensor x = as_tensor(a[0]);
+  const int format = mx_format(as_int(a[1]));
+  int launches = 0;
+  Mx q;
+  { NO_GIL; q = mx_quantize(x, format, &launches); }
+  count_launches(launches);
+  return pair_of(q.codes, q.scales);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_mx_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  ARGS(5, "mx_dequantize");
+  const Tensor codes = as_tensor(a[0]), scales = as_tensor(a[1]);
+  const int64_t cols = as_int(a[2]);
+  const int format = mx_format(as_int(a[3]));
+  const at::ScalarType dt = as_dtype(a[4]);
+  int launches = 0;
+  Tensor y;
+  { NO_GIL; y = mx_dequantize(codes, scales, cols, format, dt, &launches); }
+  count_launches(launches);
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_mx_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  ARGS(9, "mx_linear");
+  const Tensor x = as_tensor(a[0]), codes = as_tensor(a[1]), scales = as_tensor(a[2]);
+  const OptTensor bias = as_opt_tensor(a[3]), residual = as_opt_tensor(a[8]);
+  const int64_t out_f = as_int(a[4]), in_f = as_int(a[5]);
+  const at::ScalarType dt = as_dtype(a[6]);
+  const int epilogue = static_cast<int>(as_int(a[7]));
+  int launches = 0;
+  Tensor y;
+  { NO_GIL; y = mx_linear(x, codes, scales, bias, out_f, in_f, dt, epilogue, residual, &launches); }
+  count_launches(launches);
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* tuple_of(const std::vector<OptTensor>& v) {
+  PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(v.size()));
+  if (t == nullptr) return nullptr;
+  for (size_t i = 0; i < v.size(); ++i) {
+    PyObject* o = wrap(v[i]);
+    if (o == nullptr) { Py_DECREF(t); return nullptr; }
+    PyTuple_SET_ITEM(t, static_cast<Py_ssize_t>(i), o);
+  }
+  return t;
+}
+
+PyObject* py_mx_layer_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  ARGS(4, "mx_layer_forward");
+  const Tensor x = as_tensor(a[0]), weight = as_tensor(a[1]);
+  const OptTensor bias = as_opt_tensor(a[2]);
+  const int64_t k = as_int(a[3]);
+  const int keep = k == 0 ? 0 : mx_format(k);
+  int launches = 0;
+  MxForward f;
+  { NO_GIL; f = mx_layer_forward(x, weight, bias, keep, &launches); }
+  count_launches(launches);
+  return tuple_of({f.y, f.x_codes, f.x_scales, f.w.codes, f.w.scales});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_mx_grad_input(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  ARGS(5, "mx_grad_input");
+  const Tensor dy = as_tensor(a[0]), codes = as_tensor(a[1]), scales = as_tensor(a[2]);
+  const int64_t k = as_int(a[3]);
+  const at::ScalarType dt = as_dtype(a[4]);
+  int launches = 0;
+  Tensor dx;
+  { NO_GIL; dx = mx_grad_input(dy, codes, scales, k, dt, &launches); }
+  count_launches(launches);
+  return THPVariable_Wrap(dx);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_mx_grad_weight(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  ARGS(7, "mx_grad_weight");
+  const Tensor dy = as_tensor(a[0]), codes = as_tensor(a[1]), scales = as_tensor(a[2]);
+  const int64_t k = as_int(a[3]);
+  const int format = mx_format(as_int(a[4]));
+  std::optional<at::ScalarType> dw, db;
+  if (a[5] != Py_None) dw = as_dtype(a[5]);
+  if (a[6] != Py_None) db = as_dtype(a[6]);
+  int launches = 0;
+  std::pair<OptTensor, OptTensor> g;
+  { NO_GIL; g = mx_grad_weight(dy, codes, scales, k, format, dw, db, &launches); }
+  count_launches(launches);
+  return pair_of(g.first, g.second);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_mx_column_sum(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  ARGS(2, "mx_column_sum");
+  const Tensor dy = as_tensor(a[0]);
+  const at::ScalarType dt = as_dtype(a[1]);
+  int launches = 0;
+  Tensor db;
+  { NO_GIL; db = mx_column_sum(dy, dt, &launches); }
+  count_launches(launches);
+  return THPVariable_Wrap(db);
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- torch.ops.dimq: the kernels of the CUDA key for the schemas dimq_b200/ops.py defines ---------------
 // (the dispatcher calls these without the GIL)
 
@@ -1085,6 +1432,8 @@ PyObject* py_capturing(PyObject*, PyObject* device) {
 PyMethodDef kMethods[] = {FAST(linear_wq), FAST(linear_a4), FAST(conv2d_wq), FAST(conv2d_a4),
                           FAST(hard_quantize), FAST(fake_quantize_ste), FAST(unpack_bits), FAST(pack_bits), FAST(add_layer_norm),
                           FAST(max_pool_nhwc), FAST(images_to_nhwc), FAST(attention_qkv),
+                          FAST(mx_quantize), FAST(mx_dequantize), FAST(mx_linear), FAST(mx_layer_forward), FAST(mx_grad_input),
+                          FAST(mx_grad_weight), FAST(mx_column_sum),
                           {"set_launch_count", py_set_launch_count, METH_O, nullptr},
                           {"set_ops", py_set_ops, METH_O, nullptr},
                           {"record_event", py_record_event, METH_O, nullptr},

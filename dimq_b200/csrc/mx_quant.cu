@@ -1,0 +1,284 @@
+// Quantisation to microscaled blocks and back (mx_common.cuh has the formats).  Both are one pass over memory: four
+// lanes hold a block, eight values each, its largest magnitude takes two shuffles, and the rest is conversions.
+//
+// A warp takes the same 256 features of the rows r, r + 32, r + 64 and r + 96 of a row tile: four loads of 16 bytes a
+// lane in flight (fp32: eight), and the scale bytes of the four rows are the 16 that lie together in the tile.
+#include "mx_common.cuh"
+
+namespace dimq {
+namespace {
+
+using namespace mx;
+
+constexpr int kThreads = 256;
+constexpr int kSpan = 256;        // features a warp takes at a time
+constexpr int kRowsPerBlock = 8;  // rows r of one row tile, each with its three rows 32 further
+
+template <typename T>
+struct Eight {   // eight consecutive values as they are loaded
+  uint4 q[sizeof(T) / 2];
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t k, int64_t cols, float (&v)[8]) {
+  constexpr int kPer = 16 / sizeof(T);   // values per 16 bytes; rows are whole 16-byte pieces where VEC
+  if (VEC) {
+    Eight<T> e;
+#pragma unroll
+    for (int i = 0; i < 8 / kPer; ++i) {
+      e.q[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (k + i * kPer < cols) e.q[i] = __ldg(reinterpret_cast<const uint4*>(row + k + i * kPer));
+    }
+    const T* p = reinterpret_cast<const T*>(&e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_float<T>(p[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < cols ? to_float<T>(row[k + i]) : 0.0f;
+  }
+}
+
+// the four bytes of a half warp's blocks in one word, known to all its lanes
+__device__ __forceinline__ uint32_t gather_bytes(uint32_t b, int lane) {
+  uint32_t w = b << (8 * ((lane >> 2) & 3));
+  w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+  w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
+  return w;
+}
+
+// C4 / C8: the formats written
+template <typename T, bool VEC, bool C4, bool C8>
+__global__ void __launch_bounds__(kThreads)
+mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t spans, uint8_t* __restrict__ codes4,
+                   uint8_t* __restrict__ scales4, uint8_t* __restrict__ codes8, uint8_t* __restrict__ scales8) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t group = static_cast<int64_t>(blockIdx.x) / spans, span = static_cast<int64_t>(blockIdx.x) - group * spans;
+  const int64_t tile = group >> 2;
+  const int r = static_cast<int>(group & 3) * kRowsPerBlock + warp;
+  const int64_t row0 = tile * 128 + r;
+  const int64_t k = span * kSpan + lane * 8;
+  const int64_t blocks = blocks_of(cols), tiles = block_tiles(cols);
+  float v[4][8];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (row0 + 32 * q < rows) {
+      load8<T, VEC>(x + (row0 + 32 * q) * cols, k, cols, v[q]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[q][i] = 0.0f;
+    }
+  }
+  uint32_t s4[4], s8[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[q][i]) & 0x7FFFFFFFu);
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    const int64_t row = row0 + 32 * q;
+    const bool write = row < rows && k < blocks * kBlock;
+    if (C4) {
+      const uint32_t b = scale_byte(top, 2);
+      const float f = inverse_scale(b);
+      uint32_t w = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w |= encode_fp4_pair(v[q][2 * i] * f, v[q][2 * i + 1] * f) << (8 * i);
+      if (b == 255u) w = 0u;
+      if (write) *reinterpret_cast<uint32_t*>(codes4 + row * blocks * 16 + (k >> 1)) = w;
+      s4[q] = gather_bytes(b, lane);
+    }
+    if (C8) {
+      const uint32_t b = scale_byte(top, 0);
+      const float f = inverse_scale(b);
+      uint32_t w[2] = {0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = __float2int_rn(fminf(fmaxf(v[q][i] * f * 64.0f, -127.0f), 127.0f));
+        w[i >> 2] |= (static_cast<uint32_t>(c) & 0xFFu) << (8 * (i & 3));
+      }
+      if (b == 255u) w[0] = w[1] = 0u;
+      if (write) *reinterpret_cast<uint2*>(codes8 + row * blocks * 32 + k) = make_uint2(w[0], w[1]);
+      s8[q] = gather_bytes(b, lane);
+    }
+  }
+  const int64_t block_tile = span * 2 + (lane >> 4);
+  if ((lane & 15) == 0 && block_tile < tiles) {
+    const int64_t at = (tile * tiles + block_tile) * kTileBytes + r * 16;
+    if (C4) *reinterpret_cast<uint4*>(scales4 + at) = make_uint4(s4[0], s4[1], s4[2], s4[3]);
+    if (C8) *reinterpret_cast<uint4*>(scales8 + at) = make_uint4(s8[0], s8[1], s8[2], s8[3]);
+  }
+}
+
+// out rows of `pitch` values: the `cols` of the row, then zeros up to `fill`
+template <typename T, bool VEC, bool FP4>
+__global__ void __launch_bounds__(kThreads)
+mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
+                     int64_t spans, T* __restrict__ out, int64_t pitch, int64_t fill) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t group = static_cast<int64_t>(blockIdx.x) / spans, span = static_cast<int64_t>(blockIdx.x) - group * spans;
+  const int64_t tile = group >> 2;
+  const int r = static_cast<int>(group & 3) * kRowsPerBlock + warp;
+  const int64_t row0 = tile * 128 + r;
+  const int64_t k = span * kSpan + lane * 8;
+  const int64_t blocks = blocks_of(cols), tiles = block_tiles(cols);
+  const bool have = k < blocks * kBlock;
+  uint2 w[4];
+  uint32_t s[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    w[q] = make_uint2(0u, 0u);
+    const int64_t row = row0 + 32 * q;
+    if (have && row < rows) {
+      if (FP4) w[q].x = __ldg(reinterpret_cast<const uint32_t*>(codes + row * blocks * 16 + (k >> 1)));
+      else w[q] = __ldg(reinterpret_cast<const uint2*>(codes + row * blocks * 32 + k));
+    }
+  }
+  if (have) {
+    const uint4 t = __ldg(reinterpret_cast<const uint4*>(scales + (tile * tiles + span * 2 + (lane >> 4)) * kTileBytes + r * 16));
+    const int sh = 8 * ((lane >> 2) & 3);
+    s[0] = (t.x >> sh) & 0xFFu; s[1] = (t.y >> sh) & 0xFFu; s[2] = (t.z >> sh) & 0xFFu; s[3] = (t.w >> sh) & 0xFFu;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int64_t row = row0 + 32 * q;
+    if (row >= rows || k >= fill) continue;
+    float v[8];
+    if (FP4) decode_fp4(w[q].x, v);
+    else decode_int8(w[q], v);
+    const float f = scale_of(s[q]);
+    T o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = from_float<T>(k + i < cols ? v[i] * f : 0.0f);
+    T* dst = out + row * pitch + k;
+    if (VEC && k + 8 <= fill) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+        uint4 u;
+        T* p = reinterpret_cast<T*>(&u);
+#pragma unroll
+        for (int j = 0; j < 16 / static_cast<int>(sizeof(T)); ++j) p[j] = o[i * (16 / static_cast<int>(sizeof(T))) + j];
+        reinterpret_cast<uint4*>(dst)[i] = u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < fill) dst[i] = o[i];
+    }
+  }
+}
+
+int grid_of(int64_t rows, int64_t width, int64_t* spans, unsigned* grid) {
+  *spans = (width + kSpan - 1) / kSpan;
+  const int64_t g = row_tiles(rows) * 4 * *spans;
+  if (g > 0x7FFFFFFF) return DIMQ_ERR_TOO_LARGE;
+  *grid = static_cast<unsigned>(g);
+  return DIMQ_OK;
+}
+
+template <typename T>
+int quantize_as(const void* x, int64_t rows, int64_t cols, void* c4, uint8_t* s4, void* c8, uint8_t* s8, cudaStream_t st) {
+  int64_t spans;
+  unsigned grid;
+  // whole tiles of 4 blocks, so that the padding's scale bytes are written too
+  const int rc = grid_of(rows, block_tiles(cols) * 128, &spans, &grid);
+  if (rc != DIMQ_OK) return rc;
+  const T* in = static_cast<const T*>(x);
+  uint8_t *o4 = static_cast<uint8_t*>(c4), *o8 = static_cast<uint8_t*>(c8);
+  const bool vec = aligned(x, 16) && (cols * static_cast<int64_t>(sizeof(T))) % 16 == 0;
+#define DIMQ_MX_Q(V, A, B) mx_quantize_kernel<T, V, A, B><<<grid, kThreads, 0, st>>>(in, rows, cols, spans, o4, s4, o8, s8)
+  if (c4 != nullptr && c8 != nullptr) { if (vec) DIMQ_MX_Q(true, true, true); else DIMQ_MX_Q(false, true, true); }
+  else if (c4 != nullptr) { if (vec) DIMQ_MX_Q(true, true, false); else DIMQ_MX_Q(false, true, false); }
+  else { if (vec) DIMQ_MX_Q(true, false, true); else DIMQ_MX_Q(false, false, true); }
+#undef DIMQ_MX_Q
+  return launch_status();
+}
+
+template <typename T>
+int dequantize_as(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out, int64_t pitch,
+                  int64_t fill, cudaStream_t st) {
+  int64_t spans;
+  unsigned grid;
+  const int rc = grid_of(rows, fill, &spans, &grid);
+  if (rc != DIMQ_OK) return rc;
+  const uint8_t* in = static_cast<const uint8_t*>(codes);
+  T* o = static_cast<T*>(out);
+  const bool vec = aligned(out, 16) && (pitch * static_cast<int64_t>(sizeof(T))) % 16 == 0;
+#define DIMQ_MX_D(V, F) mx_dequantize_kernel<T, V, F><<<grid, kThreads, 0, st>>>(in, scales, rows, cols, spans, o, pitch, fill)
+  if (format == DIMQ_MX_FP4) { if (vec) DIMQ_MX_D(true, true); else DIMQ_MX_D(false, true); }
+  else { if (vec) DIMQ_MX_D(true, false); else DIMQ_MX_D(false, false); }
+#undef DIMQ_MX_D
+  return launch_status();
+}
+
+}  // namespace
+
+// x -> 4-bit codes, 8-bit codes, or both from one read (null: not wanted)
+int mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, void* c4, uint8_t* s4, void* c8, uint8_t* s8,
+                cudaStream_t st) {
+  if (x_dtype == DIMQ_F32) return quantize_as<float>(x, rows, cols, c4, s4, c8, s8, st);
+  if (x_dtype == DIMQ_F16) return quantize_as<__half>(x, rows, cols, c4, s4, c8, s8, st);
+  return quantize_as<__nv_bfloat16>(x, rows, cols, c4, s4, c8, s8, st);
+}
+
+int mx_dequantize(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out, int out_dtype,
+                  int64_t pitch, int64_t fill, cudaStream_t st) {
+  if (out_dtype == DIMQ_F32) return dequantize_as<float>(codes, scales, format, rows, cols, out, pitch, fill, st);
+  if (out_dtype == DIMQ_F16) return dequantize_as<__half>(codes, scales, format, rows, cols, out, pitch, fill, st);
+  return dequantize_as<__nv_bfloat16>(codes, scales, format, rows, cols, out, pitch, fill, st);
+}
+
+}  // namespace dimq
+
+using namespace dimq;
+
+static int check_mx(int64_t rows, int64_t cols, int format) {
+  if (!mx::valid_format(format)) return DIMQ_ERR_BAD_BITS;
+  if (rows < 0 || cols <= 0) return DIMQ_ERR_BAD_SIZE;
+  if (cols > (int64_t(1) << 40) || rows > (int64_t(1) << 40) || (rows > 0 && cols > (int64_t(1) << 46) / rows)) return DIMQ_ERR_TOO_LARGE;
+  return DIMQ_OK;
+}
+
+extern "C" int dimq_mx_sizes(int64_t rows, int64_t cols, int format, int64_t* code_bytes_per_row, int64_t* scale_bytes) {
+  if (code_bytes_per_row == nullptr || scale_bytes == nullptr) return DIMQ_ERR_NULL_POINTER;
+  const int rc = check_mx(rows, cols, format);
+  if (rc != DIMQ_OK) return rc;
+  *code_bytes_per_row = mx::codes_pitch(cols, format);
+  *scale_bytes = mx::scales_bytes(rows, cols);
+  return DIMQ_OK;
+}
+
+extern "C" int dimq_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int format, void* codes,
+                                uint8_t* scales, void* stream) {
+  if (!valid_dtype(x_dtype)) return DIMQ_ERR_BAD_DTYPE;
+  const int rc = check_mx(rows, cols, format);
+  if (rc != DIMQ_OK) return rc;
+  if (rows == 0) return DIMQ_OK;
+  if (x == nullptr || codes == nullptr || scales == nullptr) return DIMQ_ERR_NULL_POINTER;
+  if (!aligned(codes, 16) || !aligned(scales, 16)) return DIMQ_ERR_ALIGNMENT;
+  const bool four = format == DIMQ_MX_FP4;
+  return mx_quantize(x, x_dtype, rows, cols, four ? codes : nullptr, four ? scales : nullptr, four ? nullptr : codes,
+                     four ? nullptr : scales, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dimq_mx_quantize_both(const void* x, int x_dtype, int64_t rows, int64_t cols, uint8_t* codes4, uint8_t* scales4,
+                                     int8_t* codes8, uint8_t* scales8, void* stream) {
+  if (!valid_dtype(x_dtype)) return DIMQ_ERR_BAD_DTYPE;
+  const int rc = check_mx(rows, cols, DIMQ_MX_INT8);
+  if (rc != DIMQ_OK) return rc;
+  if (rows == 0) return DIMQ_OK;
+  if (x == nullptr || codes4 == nullptr || scales4 == nullptr || codes8 == nullptr || scales8 == nullptr) return DIMQ_ERR_NULL_POINTER;
+  if (!aligned(codes4, 16) || !aligned(scales4, 16) || !aligned(codes8, 16) || !aligned(scales8, 16)) return DIMQ_ERR_ALIGNMENT;
+  return mx_quantize(x, x_dtype, rows, cols, codes4, scales4, codes8, scales8, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dimq_mx_dequantize(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out,
+                                  int out_dtype, void* stream) {
+  if (!valid_dtype(out_dtype)) return DIMQ_ERR_BAD_DTYPE;
+  const int rc = check_mx(rows, cols, format);
+  if (rc != DIMQ_OK) return rc;
+  if (rows == 0) return DIMQ_OK;
+  if (codes == nullptr || scales == nullptr || out == nullptr) return DIMQ_ERR_NULL_POINTER;
+  if (!aligned(codes, 16) || !aligned(scales, 16)) return DIMQ_ERR_ALIGNMENT;
+  return mx_dequantize(codes, scales, format, rows, cols, out, out_dtype, cols, cols, static_cast<cudaStream_t>(stream));
+}

@@ -213,6 +213,39 @@ class DIMQLinear(_PackedBase):
         return f"{self.in_features} -> {self.out_features}, bits={self.bits}, mode={mode}"
 
 
+class MXLinear(nn.Module):
+    """Linear layer in microscaled 4-bit numbers: the weight as codes and scales, the activations quantised in the call.
+
+    ``from_linear`` takes a float layer (a trained ``nn.Linear`` or one trained with ``qat.mx_linear``, whose forward this
+    repeats); the constructor takes what ``ops.mx_quantize(weight, "fp4")`` returns.
+    """
+
+    def __init__(self, weight_codes: torch.Tensor, weight_scales: torch.Tensor, out_features: int, in_features: int,
+                 bias: torch.Tensor | None = None, *, out_dtype: torch.dtype | None = None,
+                 epilogue: str | None = None) -> None:
+        super().__init__()
+        self.register_buffer("weight_codes", weight_codes)
+        self.register_buffer("weight_scales", weight_scales)
+        self.register_buffer("bias", bias)
+        self.out_features = int(out_features)
+        self.in_features = int(in_features)
+        self.out_dtype = out_dtype
+        self.epilogue = epilogue
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, **extra) -> "MXLinear":
+        codes, scales = ops.mx_quantize(linear.weight.detach(), "fp4")
+        bias = None if linear.bias is None else linear.bias.detach().clone()
+        return cls(codes, scales, linear.out_features, linear.in_features, bias, **extra)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        return ops.mx_linear(x, self.weight_codes, self.weight_scales, self.bias, self.out_features, self.in_features,
+                             out_dtype=self.out_dtype, epilogue=self.epilogue, residual=residual)
+
+    def extra_repr(self) -> str:
+        return f"{self.in_features} -> {self.out_features}, fp4 in blocks of 32"
+
+
 class DIMQConv2d(_PackedBase):
     """Conv2d layer backed by packed weight indices and a learned codebook."""
 

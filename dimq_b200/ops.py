@@ -597,6 +597,78 @@ def add_layer_norm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Te
     return _lib.host().add_layer_norm(x, delta, weight, bias, eps)
 
 
+# ---------------------------------------------------------------------------
+# microscaled numbers: blocks of 32 values along the last dimension share a power of two
+# ---------------------------------------------------------------------------
+
+_MX_FORMATS = {"fp4": 4, "int8": 8}
+
+
+def _mx_format(fmt: str) -> int:
+    try:
+        return _MX_FORMATS[fmt]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown microscaled format {fmt!r}: 'fp4' or 'int8'") from None
+
+
+def mx_quantize(x: torch.Tensor, fmt: str = "fp4") -> tuple[torch.Tensor, torch.Tensor]:
+    """``(codes, scales)`` of ``x`` (fp32 / fp16 / bf16) in blocks of 32 values along its last dimension.
+
+    A block has the exponent ``E = max(floor(log2(max|v|)) - emax, -127)``; its values become codes of ``v * 2**-E``,
+    rounded to nearest even and saturated:
+
+    * ``"fp4"``: e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 with sign), ``emax = 2``; codes uint8, two to a byte (the first in the
+      low half), ``[..., 16 * ceil(n / 32)]``;
+    * ``"int8"``: multiples of 1/64 up to 127/64, ``emax = 0``; codes int8, ``[..., 32 * ceil(n / 32)]``.
+
+    Codes behind the last value are zero.  A block with a NaN or an infinity reads back as NaN.  ``scales`` holds the bytes
+    ``E + 127`` of all rows in tiles of 128 rows by 4 blocks, as the tensor cores take them (:func:`mx_scale_rows` gives
+    them row by row).
+    """
+    return _lib.host().mx_quantize(x, _mx_format(fmt))
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, features: int, fmt: str = "fp4", *,
+                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The values ``[..., features]`` (fp32 unless ``out_dtype``) that :func:`mx_quantize`'s codes and scales stand for."""
+    return _lib.host().mx_dequantize(codes, scales, features, _mx_format(fmt), out_dtype)
+
+
+def mx_scale_rows(scales: torch.Tensor, rows: int, features: int) -> torch.Tensor:
+    """Scale bytes row by row, ``[rows, ceil(features / 32)]``, from the tiles that :func:`mx_quantize` returns."""
+    tiles_r, tiles_b = (rows + 127) // 128, (features + 127) // 128
+    if scales.shape != (tiles_r, tiles_b, 512):
+        raise RuntimeError(f"scales must be [{tiles_r}, {tiles_b}, 512] for {rows} rows of {features} values")
+    flat = scales.view(tiles_r, tiles_b, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(tiles_r * 128, tiles_b * 4)
+    return flat[:rows, :(features + 31) // 32]
+
+
+def mx_linear(x: torch.Tensor, weight_codes: torch.Tensor, weight_scales: torch.Tensor, bias: torch.Tensor | None,
+              out_features: int, in_features: int, *, out_dtype: torch.dtype | None = None, epilogue: str | None = None,
+              residual: torch.Tensor | None = None) -> torch.Tensor:
+    """Microscaled 4-bit linear: ``q(x) @ w.T + bias`` on the 4-bit tensor cores, fp32 sums.
+
+    ``q(x)`` is ``x`` rounded by ``mx_quantize(x, "fp4")``; ``weight_codes`` / ``weight_scales`` are what
+    ``mx_quantize(weight, "fp4")`` returns for the ``[out_features, in_features]`` weight.  Output type, epilogue and
+    residual as in :func:`dimq_linear_wq`.
+    """
+    return _lib.host().mx_linear(x, weight_codes, weight_scales, bias, out_features, in_features, out_dtype,
+                                 _EPILOGUES[epilogue], residual)
+
+
+def mx_linear_grad_input(grad: torch.Tensor, weight_codes: torch.Tensor, weight_scales: torch.Tensor, in_features: int, *,
+                         out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``grad @ w`` for the 4-bit weight of :func:`mx_linear`: the gradient of its input, straight through the rounding."""
+    return _lib.host().mx_grad_input(grad, weight_codes, weight_scales, in_features, out_dtype)
+
+
+def mx_linear_grad_weight(grad: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, in_features: int,
+                          fmt: str = "int8", *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``grad.T @ x`` (over all leading dimensions) for the activations that ``mx_quantize(x, fmt)`` keeps in
+    ``codes`` / ``scales``: the gradient of a linear layer's weight, ``[out_features, in_features]``."""
+    return _lib.host().mx_grad_weight(grad, codes, scales, in_features, _mx_format(fmt), out_dtype or torch.float32, None)[0]
+
+
 def last_device_status() -> int:
     """Status word left by a tensor-core kernel that gave up a bounded wait (0 = none); clears it."""
     require_extension()

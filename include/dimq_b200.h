@@ -343,6 +343,54 @@ DIMQ_API int dimq_conv2d_a4(const void* x, int x_dtype, const dimq_wq_weight* w,
                             const dimq_conv_geom* geom, int epilogue, void* workspace, int64_t workspace_bytes,
                             void* stream);
 
+/* ---- microscaled (MX) numbers ------------------------------------------- */
+
+/* Blocks of 32 consecutive values of a row share a power of two 2^E, E = max(floor(log2 max|v|) - emax, -127), stored as
+ * the byte E + 127 (255: the block held a NaN or an infinity and reads as NaN); a value is a code times 2^E, rounded to
+ * nearest even and saturated.
+ *   DIMQ_MX_FP4   e2m1 codes, two to a byte (the first in the low half), emax = 2
+ *   DIMQ_MX_INT8  two's complement with 6 fraction bits, -127/64 .. 127/64, emax = 0
+ * Code rows hold whole blocks: ceil(cols / 32) * 16 (32) bytes, zero codes behind the last value.  Scale bytes lie in
+ * tiles of 128 rows x 4 blocks, [ceil(rows/128)][ceil(cols/128)][row % 32][row / 32 % 4][block % 4], zero where padded.
+ * Both arrays are 16-byte aligned.  The reference has no counterpart: its activations have one scale per tensor. */
+#define DIMQ_MX_FP4 4
+#define DIMQ_MX_INT8 8
+
+/* Bytes of one row of codes, and of all scales, of a [rows][cols] matrix. */
+DIMQ_API int dimq_mx_sizes(int64_t rows, int64_t cols, int format, int64_t* code_bytes_per_row, int64_t* scale_bytes);
+
+/* x [rows][cols] (any of the three types, contiguous) -> codes and scales. */
+DIMQ_API int dimq_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int format, void* codes,
+                              uint8_t* scales, void* stream);
+
+/* The same to both formats from one read of x. */
+DIMQ_API int dimq_mx_quantize_both(const void* x, int x_dtype, int64_t rows, int64_t cols, uint8_t* codes4, uint8_t* scales4,
+                                   int8_t* codes8, uint8_t* scales8, void* stream);
+
+/* codes and scales -> out [rows][cols]. */
+DIMQ_API int dimq_mx_dequantize(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out,
+                                int out_dtype, void* stream);
+
+/* y [M][N] = epilogue(x^ w^T + bias) + residual, x^ the DIMQ_MX_FP4 values of x [M][K], w^ those of w_codes / w_scales
+ * ([N][K]), products and sums in fp32.  Bias, epilogue and residual as in dimq_linear_wq (residual: y's type).  With
+ * x_scales != NULL, x holds the codes of x^ already (x_dtype is not looked at).  Scratch:
+ * dimq_mx_linear_workspace_bytes (coded: whether x_scales is given), 16-byte aligned. */
+DIMQ_API int dimq_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int coded, int64_t* bytes);
+DIMQ_API int dimq_mx_linear(const void* x, int x_dtype, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales,
+                            const void* bias, int bias_dtype, const void* residual, void* y, int y_dtype, int64_t M, int64_t N,
+                            int64_t K, int epilogue, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients of that layer, straight through the quantisation: dx [M][K] = dy w^ and dw [N][K] = dy^T x~, db [N] the column
+ * sums of dy [M][N] (dw or db may be NULL; without dw nothing of x is read).  x~ is what x_codes / x_scales hold (either format: the 8-bit copy is what a layer
+ * keeps of its activations).  dy is taken exactly, sums in fp32.  Scratch for both: dimq_mx_grad_workspace_bytes. */
+DIMQ_API int dimq_mx_grad_workspace_bytes(int dy_dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes);
+DIMQ_API int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, void* dx,
+                                int dx_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                                void* stream);
+DIMQ_API int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_codes, const uint8_t* x_scales, int format, void* dw,
+                                 int dw_dtype, void* db, int db_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
 /* ---- dense helper of the whole-model harness --------------------------- */
 
 /* out[b][t][h][:] = softmax(scale * q k^T) v per batch b and head h, for qkv [batch][tokens][3][heads][64] (DIMQ_BF16 or
