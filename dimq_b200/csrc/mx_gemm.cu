@@ -1,8 +1,15 @@
-// Products of microscaled matrices: y = x^ w^T, and the two gradients of that layer.
+// The microscaled 4-bit product y = x^ w^T on the block-scaled tensor cores.
 //
-// One plain kernel for all three: 64 x 64 tiles of the result, 16 of the reduction at a time decoded to fp32 in shared
-// memory, 4 x 4 results a thread.
-#include "mx_common.cuh"
+// tcgen05.mma kind::mxf4 multiplies e2m1 codes as they are stored, 64 of them a step, and scales each block of 32 by the
+// two operands' powers of two before it adds: products and scaling are exact, sums are fp32.  So nothing is decoded: TMA
+// brings codes (rows of 128 bytes = 256 values, 128-byte swizzle) and the 512-byte scale tiles that the format keeps,
+// tcgen05.cp moves a scale tile to tensor memory, and the accumulators go through bias, activation and residual to y.
+//
+// Tile: 128 rows of x (one tensor-memory lane each) x BN rows of w.  A ring stage holds 256 k of both operands and their
+// scales; its scale columns in tensor memory belong to the stage too, so the commit that frees the stage frees them.
+// Warps 0-2 fetch (they take the stages in turn), warp 3 issues copies and MMAs, warps 4-11 are the epilogue: two to each
+// quarter of the lanes, taking 32-column pieces in turn.  Persistent grid, one block per SM.
+#include "mx_tile.cuh"
 
 namespace dimq {
 int mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, void* c4, uint8_t* s4, void* c8, uint8_t* s8,
@@ -12,93 +19,317 @@ namespace {
 
 using namespace mx;
 
-struct Coded {   // a microscaled matrix [rows][cols]
-  const uint8_t* codes;
-  const uint8_t* scales;
-  int64_t blocks, tiles;
-  int fp4;
-  __device__ float at(int64_t r, int64_t k) const {
-    const float f = scale_of(scales[scale_offset(r, k >> 5, tiles)]);
-    float v[8];
-    if (fp4) {
-      decode_fp4(codes[r * blocks * 16 + (k >> 1)] >> (4 * (k & 1)), v);
-      return v[0] * f;
-    }
-    return static_cast<float>(static_cast<int8_t>(codes[r * blocks * 32 + k])) * 0.015625f * f;
-  }
-};
-Coded coded(const void* codes, const uint8_t* scales, int64_t cols, int format) {
-  return {static_cast<const uint8_t*>(codes), scales, blocks_of(cols), block_tiles(cols), format == DIMQ_MX_FP4};
-}
+constexpr int kProducers = 3;
+constexpr int kThreads = (kProducers + 1 + kEpiWarps) * 32;
+constexpr int kMaxStages = 8;
+constexpr int kSfCol = 256;                      // first tensor-memory column of the scales
+constexpr uint32_t kABytes = 128 * 128;
+constexpr int kSegStages = 8;                    // fp32 results: sums of 2048 k are added up in registers
 
-struct Dense {
-  const void* p;
-  int dtype;
-  int64_t cols;
-  __device__ float at(int64_t r, int64_t k) const { return load_as_float(p, dtype, r * cols + k); }
+struct GemmMaps {
+  CUtensorMap a, b, y;
 };
 
-// c[r][j] = sum_t A(r, t) B(t, j); AT / BT: the operand is stored with its axes exchanged
-template <typename A, bool AT, typename B, bool BT>
-__global__ void __launch_bounds__(256)
-mx_plain_kernel(A a, B b, int64_t R, int64_t J, int64_t T, const void* bias, int bias_dtype, const void* residual, void* c,
-                int c_dtype, int epilogue) {
-  __shared__ float sa[16][65], sb[16][65];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, j0 = static_cast<int64_t>(blockIdx.x) * 64;
-  float acc[4][4] = {};
-  for (int64_t t0 = 0; t0 < T; t0 += 16) {
-    for (int i = threadIdx.x; i < 1024; i += 256) {
-      const int t = AT ? i >> 6 : i & 15, r = AT ? i & 63 : i >> 4;
-      const bool in = r0 + r < R && t0 + t < T;
-      sa[t][r] = in ? (AT ? a.at(t0 + t, r0 + r) : a.at(r0 + r, t0 + t)) : 0.0f;
-      const int tb = BT ? i & 15 : i >> 6, j = BT ? i >> 4 : i & 63;
-      const bool inb = j0 + j < J && t0 + tb < T;
-      sb[tb][j] = inb ? (BT ? b.at(j0 + j, t0 + tb) : b.at(t0 + tb, j0 + j)) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < 16; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[t][ty + 16 * i], sb[t][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = r0 + ty + 16 * i, k = j0 + tx + 16 * j;
-      if (r >= R || k >= J) continue;
-      float v = acc[i][j];
-      if (bias != nullptr) v += load_as_float(bias, bias_dtype, k);
-      v = finish_value(v, epilogue, residual != nullptr, residual != nullptr ? load_as_float(residual, c_dtype, r * J + k) : 0.0f);
-      store_from_float(c, c_dtype, r * J + k, v);
-    }
+struct GemmParams {
+  const uint8_t *sfa, *sfb;
+  Out out;
+  int k_tiles;             // scale tiles along k (128 values each)
+  int row_tiles_b;         // scale tiles along n
+  int stages, n_tiles, tiles;
+};
+
+struct GemmHeader {
+  uint64_t full[kMaxStages], empty[kMaxStages], d_full[2], d_empty[2];
+  uint32_t tmem_base;
+  volatile uint32_t abort_flag;
+};
+
+// scale tile (32 rows x 16 bytes) -> 4 columns, the same in all four lane quarters
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// rows of 16 bytes, eight to a 128-byte group, no swizzle
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem) {
+  return static_cast<uint64_t>((smem & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// e2m1 times e2m1 with e8m0 scales; `half`: which two of the four scale bytes of a column belong to this step
+__host__ __device__ constexpr uint32_t mxf4_idesc(int m, int n, int half) {
+  return (static_cast<uint32_t>(2 * half) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(m >> 7) << 27) | (static_cast<uint32_t>(2 * half) << 29);
 }
 
-__global__ void __launch_bounds__(256)
-mx_column_sum_kernel(Dense a, int64_t rows, void* out, int out_dtype) {
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
-  __shared__ float part[8][32];
-  float s = 0.0f;
-  if (j < a.cols)
-    for (int64_t r = threadIdx.x >> 5; r < rows; r += 8) s += a.at(r, j);
-  part[threadIdx.x >> 5][threadIdx.x & 31] = s;
+template <int BN>
+struct Shape {
+  static constexpr int kRowTiles = BN > 128 ? BN / 128 : 1;               // scale tiles of w a stage holds per k tile
+  static constexpr uint32_t kBBytes = BN * 128;
+  static constexpr uint32_t kStageBytes = kABytes + kBBytes + 1024 + kRowTiles * 1024;
+  static constexpr int kSfCols = 8 + 8 * kRowTiles;                      // tensor-memory columns of a stage's scales
+  static constexpr int kBufs = BN > 128 ? 1 : 2;                         // accumulators
+  static constexpr int kMost = (512 - kSfCol) / kSfCols < kMaxStages ? (512 - kSfCol) / kSfCols : kMaxStages;
+};
+
+template <int BN, int ES, bool SEG>
+__global__ void __launch_bounds__(kThreads, 1)
+mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
+  using S = Shape<BN>;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t n_st = static_cast<uint32_t>(p.stages);
+  GemmHeader* hdr = reinterpret_cast<GemmHeader*>(smem + n_st * S::kStageBytes);
+  unsigned char* staging = reinterpret_cast<unsigned char*>(hdr) + kHeaderBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k_stages = (p.k_tiles + 1) / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), kEpiWarps); }
+    hdr->abort_flag = 0u;
+    fence_barrier_init();
+    prefetch_tensormap(&maps.a);
+    prefetch_tensormap(&maps.b);
+    if (p.out.tma) prefetch_tensormap(&maps.y);
+  }
+  if (warp == kProducers) {
+    tmem_alloc(smem_u32(&hdr->tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
   __syncthreads();
-  if (threadIdx.x < 32 && j < a.cols) {
-    for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
-    store_from_float(out, out_dtype, j, s);
+  tc_fence_after();
+  const uint32_t tmem = hdr->tmem_base;
+  volatile uint32_t* abort_flag = &hdr->abort_flag;
+  wait_for_inputs();
+
+  if (warp < kProducers) {
+    // no more producers than stages: a warp's successive stages are at most one revolution apart, or the one bit of a
+    // barrier's phase could not tell the round it waits for from the one before
+    const uint32_t turns = n_st < kProducers ? n_st : kProducers;
+    uint32_t stage = 0, phase = 0, turn = 0, issued = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+      const int n_blk = t % p.n_tiles, m_blk = t / p.n_tiles;
+      for (int kb = 0; kb < k_stages; ++kb) {
+        if (turn == static_cast<uint32_t>(warp)) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase ^ 1u, abort_flag, 0x2100u | stage))) { ok = false; break; }
+          const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * S::kStageBytes);
+          const uint32_t sf_bytes = p.k_tiles - 2 * kb >= 2 ? 1024u : 512u;
+          const int rt0 = n_blk * BN / 128;
+          const int rts = S::kRowTiles < p.row_tiles_b - rt0 ? S::kRowTiles : p.row_tiles_b - rt0;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(full, kABytes + S::kBBytes + sf_bytes * (1 + rts));
+            tma_load_2d(dst, &maps.a, full, kb * 128, m_blk * 128);
+            tma_load_2d(dst + kABytes, &maps.b, full, kb * 128, n_blk * BN);
+            const uint32_t sf = dst + kABytes + S::kBBytes;
+            bulk_load(sf, p.sfa + (static_cast<int64_t>(m_blk) * p.k_tiles + 2 * kb) * kTileBytes, sf_bytes, full);
+            for (int i = 0; i < rts; ++i)
+              bulk_load(sf + 1024 * (1 + i), p.sfb + (static_cast<int64_t>(rt0 + i) * p.k_tiles + 2 * kb) * kTileBytes, sf_bytes, full);
+          }
+          __syncwarp();
+        }
+        ++issued;
+        if (++turn == turns) turn = 0;
+        if (++stage == n_st) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0) {   // gave up: bounded wait for the copies in flight, so that none lands after the block has gone
+      const uint32_t n_back = issued < n_st ? issued : n_st;
+      uint32_t s = stage, ph = phase;
+      for (uint32_t i = 0; i < n_back; ++i) {
+        if (s == 0) { s = n_st - 1; ph ^= 1u; } else { --s; }
+        for (uint32_t it = 0; it < kSpinLimit; ++it)
+          if (mbar_try_wait(smem_u32(&hdr->full[s]), ph)) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == kProducers) {
+    uint32_t stage = 0, phase = 0, buf = 0, bph = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+      const int n0 = (t % p.n_tiles) * BN;
+      for (int seg0 = 0; seg0 < k_stages && ok; seg0 += SEG ? kSegStages : k_stages) {
+        const int seg1 = SEG && seg0 + kSegStages < k_stages ? seg0 + kSegStages : k_stages;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_empty[buf]), bph ^ 1u, abort_flag, 0x2200u | buf))) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d = tmem + buf * 128;
+        for (int kb = seg0; kb < seg1; ++kb) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->full[stage]), phase, abort_flag, 0x2300u | stage))) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
+          const uint64_t a0 = make_smem_desc_sw128(at), b0 = make_smem_desc_sw128(at + kABytes);
+          const uint64_t sf0 = scale_desc(at + kABytes + S::kBBytes);
+          const uint32_t sfa = tmem + kSfCol + stage * S::kSfCols, sfb = sfa + 8;
+          const int kts = p.k_tiles - 2 * kb < 2 ? p.k_tiles - 2 * kb : 2;
+          if (elect_one()) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+              if (kt < kts) {   // a scale tile that is not there has no values either
+                copy_scales(sfa + 4 * kt, sf0 + static_cast<uint64_t>(kt * (kTileBytes >> 4)));
+#pragma unroll
+                for (int i = 0; i < S::kRowTiles; ++i)
+                  copy_scales(sfb + (kt * S::kRowTiles + i) * 4, sf0 + static_cast<uint64_t>((1024 * (1 + i) + kt * kTileBytes) >> 4));
+#pragma unroll
+                for (int j = 0; j < 2; ++j)   // 64 k = 32 bytes inside the swizzled row
+                  mma_mxf4(d, a0 + static_cast<uint64_t>(4 * kt + 2 * j), b0 + static_cast<uint64_t>(4 * kt + 2 * j), mxf4_idesc(128, BN, j),
+                           sfa + 4 * kt, sfb + kt * S::kRowTiles * 4 + (BN == 64 && (n0 & 64) ? 2 : 0), (kb > seg0 || kt || j) ? 1u : 0u);
+              }
+            }
+            mma_commit(smem_u32(&hdr->empty[stage]));
+          }
+          __syncwarp();
+          if (++stage == n_st) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        if (elect_one()) mma_commit(smem_u32(&hdr->d_full[buf]));
+        __syncwarp();
+        if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
+      }
+    }
+  } else {
+    const int ew = warp - kProducers - 1;
+    const int quarter = warp & 3, sub = ew >> 2;   // pieces sub, sub + 2, ... of the tile's columns
+    unsigned char* stage = staging + ew * (ES == 2 && p.out.tma ? 2048 : 4096);
+    constexpr int kChunks = BN / 32, kMine = kChunks / 2;
+    uint32_t buf = 0, bph = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+      const int64_t n_first = static_cast<int64_t>(t % p.n_tiles) * BN, row0 = static_cast<int64_t>(t / p.n_tiles) * 128 + quarter * 32;
+      float bias[kMine];
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int64_t n = n_first + (sub + 2 * i) * 32 + lane;
+        bias[i] = p.out.bias != nullptr && n < p.out.cols ? load_as_float(p.out.bias, p.out.bias_dtype, n) : 0.0f;
+      }
+      const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+      if constexpr (SEG) {
+        float sum[kMine][32];
+        for (int seg0 = 0; seg0 < k_stages; seg0 += kSegStages) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf))) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            uint32_t r[32];
+            tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[i][j] = seg0 == 0 ? __uint_as_float(r[j]) : sum[i][j] + __uint_as_float(r[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&hdr->d_empty[buf]));
+          __syncwarp();
+          if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int64_t n0 = n_first + (sub + 2 * i) * 32;
+          if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[i], p.out, &maps.y, stage, bias[i], row0, n0, lane);
+        }
+      } else {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf))) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          uint32_t r[32];
+          tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, r);
+          tmem_ld_wait();
+          if (i == kMine - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&hdr->d_empty[buf]));
+          }
+          __syncwarp();
+          const int64_t n0 = n_first + (sub + 2 * i) * 32;
+          if (row0 < p.out.rows && n0 < p.out.cols) {
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+            put_chunk<ES>(v, p.out, &maps.y, stage, bias[i], row0, n0, lane);
+          }
+        }
+        if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
+      }
+    }
+    __syncwarp();
+    if (elect_one()) tma_store_wait_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kProducers) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
-template <typename A, bool AT, typename B, bool BT>
-int plain(A a, B b, int64_t R, int64_t J, int64_t T, const void* bias, int bias_dtype, const void* residual, void* c, int c_dtype,
-          int epilogue, cudaStream_t st) {
-  const int64_t gx = (J + 63) / 64, gy = (R + 63) / 64;
-  if (gx > 0x7FFFFFFF || gy > 65535) return DIMQ_ERR_TOO_LARGE;
-  mx_plain_kernel<A, AT, B, BT><<<dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), 256, 0, st>>>(
-      a, b, R, J, T, bias, bias_dtype, residual, c, c_dtype, epilogue);
-  return launch_status();
+bool code_map(CUtensorMap* m, const void* codes, int64_t rows, int64_t K, int box_rows) {   // bytes, 128 of them a box row
+  const cuuint64_t pitch = static_cast<cuuint64_t>(codes_pitch(K, DIMQ_MX_FP4));
+  const cuuint64_t dims[2] = {pitch, static_cast<cuuint64_t>(rows)};
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+  return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, &pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int BN, int ES, bool SEG>
+int launch_gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& out, int64_t K, cudaStream_t st) {
+  using S = Shape<BN>;
+  GemmMaps maps;
+  GemmParams p = {};
+  p.sfa = xs;
+  p.sfb = ws;
+  p.out = out;
+  p.k_tiles = static_cast<int>(block_tiles(K));
+  p.row_tiles_b = static_cast<int>(row_tiles(out.cols));
+  p.n_tiles = static_cast<int>((out.cols + BN - 1) / BN);
+  const int64_t tiles = row_tiles(out.rows) * p.n_tiles;
+  if (tiles > 0x7FFFFFFF - kNumSMs) return DIMQ_ERR_TOO_LARGE;
+  p.tiles = static_cast<int>(tiles);
+  if (!code_map(&maps.a, xc, out.rows, K, 128) || !code_map(&maps.b, wc, out.cols, K, BN) || (out.tma && !encode_out(&maps.y, out)))
+    return DIMQ_ERR_DRIVER;
+  const size_t fixed = 1024 + kHeaderBytes + kEpiWarps * (ES == 2 && out.tma ? 2048 : 4096);
+  p.stages = static_cast<int>((kSmemMax - fixed) / S::kStageBytes);
+  if (p.stages > S::kMost) p.stages = S::kMost;
+  auto kern = mx_gemm_kernel<BN, ES, SEG>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const unsigned grid = static_cast<unsigned>(tiles < kNumSMs ? tiles : kNumSMs);
+  e = launch_dependent(kern, grid, kThreads, fixed + p.stages * S::kStageBytes, st, 1, maps, p);
+  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+}
+
+// Columns a tile takes: the width that needs the fewest waves of tiles, weighed by what a 256-k step of that width costs.
+int choose_bn(int64_t M, int64_t N) {
+  const int width[3] = {256, 128, 64};
+  const double cost[3] = {768.0, 520.0, 430.0};
+  int best = 64;
+  double least = 0.0;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t tiles = row_tiles(M) * ((N + width[i] - 1) / width[i]);
+    const double c = static_cast<double>((tiles + kNumSMs - 1) / kNumSMs) * cost[i];
+    if (i == 0 || c < least) { least = c; best = width[i]; }
+  }
+  return best;
+}
+
+int gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& out, int64_t K, cudaStream_t st) {
+  const bool wide = out.dtype == DIMQ_F32, seg = wide && block_tiles(K) > 2 * kSegStages;
+  const int bn = choose_bn(out.rows, out.cols);
+#define DIMQ_MX_GEMM(BN, ES, SEG) return launch_gemm<BN, ES, SEG>(xc, xs, wc, ws, out, K, st)
+  if (seg) { if (bn == 64) DIMQ_MX_GEMM(64, 4, true); DIMQ_MX_GEMM(128, 4, true); }
+  if (wide) { if (bn == 256) DIMQ_MX_GEMM(256, 4, false); if (bn == 128) DIMQ_MX_GEMM(128, 4, false); DIMQ_MX_GEMM(64, 4, false); }
+  if (bn == 256) DIMQ_MX_GEMM(256, 2, false);
+  if (bn == 128) DIMQ_MX_GEMM(128, 2, false);
+  DIMQ_MX_GEMM(64, 2, false);
+#undef DIMQ_MX_GEMM
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K) {
@@ -107,7 +338,12 @@ int check_sizes(int64_t M, int64_t N, int64_t K) {
   return DIMQ_OK;
 }
 
+int64_t codes_room(int64_t M, int64_t K) { return (codes_bytes(M, K, DIMQ_MX_FP4) + 511) / 512 * 512; }
+
 }  // namespace
+
+int read_mx_status(uint32_t* status) { return tc::read_and_clear_device_status(status); }
+
 }  // namespace dimq
 
 using namespace dimq;
@@ -117,7 +353,7 @@ extern "C" int dimq_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, i
   *bytes = 0;
   const int rc = check_sizes(M, N, K);
   if (rc != DIMQ_OK) return rc;
-  if (!coded) *bytes = (mx::codes_bytes(M, K, DIMQ_MX_FP4) + 511) / 512 * 512 + mx::scales_bytes(M, K);
+  if (!coded) *bytes = codes_room(M, K) + mx::scales_bytes(M, K);
   return DIMQ_OK;
 }
 
@@ -134,65 +370,17 @@ extern "C" int dimq_mx_linear(const void* x, int x_dtype, const uint8_t* x_scale
       (x_scales != nullptr && !aligned(x, 16)))
     return DIMQ_ERR_ALIGNMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const void* xc = x;
-  const uint8_t* xs = x_scales;
+  const uint8_t *xc = static_cast<const uint8_t*>(x), *xs = x_scales;
   if (x_scales == nullptr) {
-    int64_t need = 0;
-    dimq_mx_linear_workspace_bytes(M, N, K, 0, &need);
-    if (workspace == nullptr || workspace_bytes < need) return DIMQ_ERR_SCRATCH_TOO_SMALL;
+    if (workspace == nullptr || workspace_bytes < codes_room(M, K) + mx::scales_bytes(M, K)) return DIMQ_ERR_SCRATCH_TOO_SMALL;
     uint8_t* c = static_cast<uint8_t*>(workspace);
-    uint8_t* s = c + (mx::codes_bytes(M, K, DIMQ_MX_FP4) + 511) / 512 * 512;
+    uint8_t* s = c + codes_room(M, K);
     rc = mx_quantize(x, x_dtype, M, K, c, s, nullptr, nullptr, st);
     if (rc != DIMQ_OK) return rc;
     xc = c;
     xs = s;
   }
-  return plain<Coded, false, Coded, true>(coded(xc, xs, K, DIMQ_MX_FP4), coded(w_codes, w_scales, K, DIMQ_MX_FP4), M, N, K, bias,
-                                          bias_dtype, residual, y, y_dtype, epilogue, st);
-}
-
-extern "C" int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, void* dx,
-                                  int dx_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
-                                  void* stream) {
-  const int rc = check_sizes(M, N, K);
-  if (rc != DIMQ_OK) return rc;
-  if (!valid_dtype(dy_dtype) || !valid_dtype(dx_dtype)) return DIMQ_ERR_BAD_DTYPE;
-  if (M == 0) return DIMQ_OK;
-  if (dy == nullptr || w_codes == nullptr || w_scales == nullptr || dx == nullptr) return DIMQ_ERR_NULL_POINTER;
-  if (!aligned(w_codes, 16) || !aligned(w_scales, 16) || !aligned(workspace, 16)) return DIMQ_ERR_ALIGNMENT;
-  int64_t need = 0;
-  dimq_mx_grad_workspace_bytes(dy_dtype, M, N, K, &need);
-  if (workspace == nullptr || workspace_bytes < need) return DIMQ_ERR_SCRATCH_TOO_SMALL;
-  return plain<Dense, false, Coded, false>(Dense{dy, dy_dtype, N}, coded(w_codes, w_scales, K, DIMQ_MX_FP4), M, K, N, nullptr, 0,
-                                           nullptr, dx, dx_dtype, DIMQ_EPI_NONE, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_codes, const uint8_t* x_scales, int format, void* dw,
-                                   int dw_dtype, void* db, int db_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
-                                   int64_t workspace_bytes, void* stream) {
-  int rc = check_sizes(M, N, K);
-  if (rc != DIMQ_OK) return rc;
-  if (!mx::valid_format(format)) return DIMQ_ERR_BAD_BITS;
-  if (!valid_dtype(dy_dtype) || (dw != nullptr && !valid_dtype(dw_dtype)) || (db != nullptr && !valid_dtype(db_dtype))) return DIMQ_ERR_BAD_DTYPE;
-  if ((dw == nullptr && db == nullptr) || (M > 0 && (dy == nullptr || (dw != nullptr && (x_codes == nullptr || x_scales == nullptr))))) return DIMQ_ERR_NULL_POINTER;
-  if (!aligned(x_codes, 16) || !aligned(x_scales, 16) || !aligned(workspace, 16)) return DIMQ_ERR_ALIGNMENT;
-  int64_t need = 0;
-  dimq_mx_grad_workspace_bytes(dy_dtype, M, N, K, &need);
-  if (workspace == nullptr || workspace_bytes < need) return DIMQ_ERR_SCRATCH_TOO_SMALL;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dw != nullptr)
-    rc = plain<Dense, true, Coded, false>(Dense{dy, dy_dtype, N}, coded(x_codes, x_scales, K, format), N, K, M, nullptr, 0, nullptr, dw,
-                                        dw_dtype, DIMQ_EPI_NONE, st);
-  if (rc != DIMQ_OK || db == nullptr) return rc;
-  mx_column_sum_kernel<<<static_cast<unsigned>((N + 31) / 32), 256, 0, st>>>(Dense{dy, dy_dtype, N}, M, db, db_dtype);
-  return launch_status();
-}
-
-extern "C" int dimq_mx_grad_workspace_bytes(int dy_dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes) {
-  if (bytes == nullptr) return DIMQ_ERR_NULL_POINTER;
-  *bytes = 0;
-  if (!valid_dtype(dy_dtype)) return DIMQ_ERR_BAD_DTYPE;
-  const int rc = check_sizes(M, N, K);
-  if (rc == DIMQ_OK) *bytes = 16;
-  return rc;
+  mx::Out out = {y, residual, bias, M, N, bias_dtype, y_dtype, epilogue, 0};
+  out.tma = mx::out_by_map(out);
+  return gemm(xc, xs, w_codes, w_scales, out, K, st);
 }

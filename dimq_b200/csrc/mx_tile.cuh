@@ -1,0 +1,210 @@
+// What the microscaled products share: copies, the output of a 32 x 32 piece, the tensor-map encoder.
+#pragma once
+
+#include "mx_common.cuh"
+#include "tc_common.cuh"
+
+namespace dimq {
+namespace mx {
+
+using namespace tc;
+
+constexpr int kHeaderBytes = 1024;
+constexpr int kEpiWarps = 8;
+constexpr size_t kSmemMax = 227 * 1024;   // what a block may use: every kernel's limit is set to this, never to a call's own size
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) == cudaSuccess &&
+        qres == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(sym);
+    return static_cast<EncodeTiledFn>(nullptr);
+  }();
+  return fn;
+}
+
+// rank 2 or 3, innermost first; zero fill outside
+inline bool encode_map(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn encode = encode_tiled();
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return encode != nullptr &&
+         encode(m, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, estr,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+inline CUtensorMapDataType map_dtype(int dtype) {
+  return dtype == DIMQ_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                           : dtype == DIMQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// Launched as a programmatic dependent: the prologue overlaps the end of the kernel before it in the stream; every thread
+// of such a kernel waits (wait_for_inputs) before it touches global memory.
+template <typename Kern, typename... Args>
+cudaError_t launch_dependent(Kern kern, unsigned grid, int threads, size_t smem, cudaStream_t st, int cluster, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+template <int EPI>
+__device__ __forceinline__ float activate(float v, float res) {
+  if (EPI == DIMQ_EPI_ADD_RELU) return max_nan(v + res, 0.0f);
+  if (EPI == DIMQ_EPI_RELU) v = max_nan(v, 0.0f);
+  if (EPI == DIMQ_EPI_GELU) v = 0.5f * v * (1.0f + fast_erf(v * 0.70710678118654752440f));
+  return v + res;
+}
+__device__ __forceinline__ float activate_any(float v, float res, int epilogue) {
+  if (epilogue == DIMQ_EPI_NONE) return v + res;
+  if (epilogue == DIMQ_EPI_RELU) return activate<DIMQ_EPI_RELU>(v, res);
+  if (epilogue == DIMQ_EPI_GELU) return activate<DIMQ_EPI_GELU>(v, res);
+  return activate<DIMQ_EPI_ADD_RELU>(v, res);
+}
+
+struct Out {            // where a product goes
+  void* y;
+  const void* residual; // y's type and layout, or null
+  const void* bias;     // one per column, or null
+  int64_t rows, cols;
+  int bias_dtype, dtype, epilogue;
+  int tma;              // rows of whole 16-byte pieces: the tensor map stores them
+};
+
+template <int ES>
+__device__ __forceinline__ float element(const uint4& q, int i, int dtype) {
+  const uint32_t w = i < (ES == 2 ? 2 : 1) ? q.x : i < (ES == 2 ? 4 : 2) ? q.y : i < (ES == 2 ? 6 : 3) ? q.z : q.w;
+  if (ES == 4) return __uint_as_float(w);
+  const unsigned short h = static_cast<unsigned short>(i & 1 ? w >> 16 : w);
+  return dtype == DIMQ_BF16 ? __uint_as_float(static_cast<uint32_t>(h) << 16) : __half2float(__ushort_as_half(h));
+}
+
+// Sums of 32 rows x 32 columns (lane = row, v = its columns from n0 on) -> y.  `bias` is that of column n0 + lane.
+// stage: this warp's piece of shared memory, 1024-aligned (ES = 2 through the map: 2 KB, else 4 KB).
+// With a map: bias, activation and residual on the lane's row, packed into the swizzled box the map stores.  Without: the
+// sums change hands through shared memory, so that a warp stores 32 neighbours of one row at a time.
+template <int ES>
+__device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CUtensorMap* map, unsigned char* stage, float bias,
+                                          int64_t row0, int64_t n0, int lane) {
+  if (o.tma) {
+    const int64_t row = row0 + lane;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, bias, j);
+    if (o.residual != nullptr) {
+      constexpr int kPer = 16 / ES;
+      const char* r = static_cast<const char*>(o.residual) + (row * o.cols + n0) * ES;
+#pragma unroll
+      for (int c = 0; c < 32 / kPer; ++c) {
+        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+        if (row < o.rows && n0 + c * kPer < o.cols) q = __ldg(reinterpret_cast<const uint4*>(r) + c);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[c * kPer + i] = activate_any(v[c * kPer + i], element<ES>(q, i, o.dtype), o.epilogue);
+      }
+    } else if (o.epilogue == DIMQ_EPI_GELU) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = activate<DIMQ_EPI_GELU>(v[j], 0.0f);
+    } else if (o.epilogue != DIMQ_EPI_NONE) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = max_nan(v[j], 0.0f);
+    }
+    if (elect_one()) tma_store_wait_read();   // the last store has read this piece
+    __syncwarp();
+    if (ES == 2) {   // 64-byte rows, 64-byte swizzle
+      unsigned char* p = stage + lane * 64;
+      const int sw = (lane >> 1) & 3;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a = v[8 * j + 2 * i], b = v[8 * j + 2 * i + 1];
+          if (o.dtype == DIMQ_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(b), "f"(a));
+          else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(b), "f"(a));
+        }
+        *reinterpret_cast<uint4*>(p + ((j ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    } else {         // 128-byte rows, 128-byte swizzle
+      unsigned char* p = stage + lane * 128;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<float4*>(p + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (elect_one()) {
+      tma_store_2d(map, smem_u32(stage), static_cast<int>(n0), static_cast<int>(row0));
+      tma_store_commit();
+    }
+    __syncwarp();
+    return;
+  }
+  float* f = reinterpret_cast<float*>(stage);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) f[lane * 32 + (j ^ lane)] = v[j];
+  __syncwarp();
+  const int64_t n = n0 + lane;
+  if (n < o.cols) {
+    const int rows = static_cast<int>(o.rows - row0 < 32 ? o.rows - row0 : 32);
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      const int64_t at = (row0 + r) * o.cols + n;
+      const float res = o.residual != nullptr ? load_as_float(o.residual, o.dtype, at) : 0.0f;
+      store_from_float(o.y, o.dtype, at, activate_any(f[r * 32 + (lane ^ r)] + bias, res, o.epilogue));
+    }
+  }
+  __syncwarp();
+}
+
+#endif
+
+inline bool out_by_map(const Out& o) {
+  const int64_t es = o.dtype == DIMQ_F32 ? 4 : 2;
+  return aligned(o.y, 16) && (o.residual == nullptr || aligned(o.residual, 16)) && (o.cols * es) % 16 == 0;
+}
+inline bool encode_out(CUtensorMap* m, const Out& o) {   // boxes of 32 rows x 32 columns
+  const cuuint64_t es = o.dtype == DIMQ_F32 ? 4 : 2;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(o.cols), static_cast<cuuint64_t>(o.rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(o.cols) * es};
+  const cuuint32_t box[2] = {32, 32};
+  return encode_map(m, map_dtype(o.dtype), 2, o.y, dims, strides, box, es == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+}  // namespace mx
+}  // namespace dimq

@@ -135,7 +135,8 @@ def _check_linear(y, x4, w4, bias, epilogue, residual, out_dtype):
 
 
 LINEAR = [(1, 1, 1), (1, 32, 8), (3, 33, 7), (2, 100, 128), (8, 256, 130), (16, 1000, 129), (17, 1024, 64), (1, 4096, 256), (5, 8320, 128),
-          (33, 520, 257), (64, 2050, 100), (128, 128, 128), (130, 300, 257), (197, 768, 96), (300, 1001, 515), (257, 512, 640)]
+          (33, 520, 257), (64, 2050, 100), (128, 128, 128), (130, 300, 257), (197, 768, 96), (300, 1001, 515), (257, 512, 640),
+          (2500, 330, 2568), (1300, 4420, 2600)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -183,6 +184,9 @@ def test_linear_non_finite_and_extreme_blocks(cuda_device, m, k, n):
     y = ops.mx_linear(x, codes, scales, None, n, k)
     assert torch.equal(y.isnan().any(0).cpu().nonzero().flatten(), torch.arange(n))     # row 1
     _check_linear(y, x4, w4, None, None, None, torch.float32)
+    for epilogue in ("relu", "gelu"):                       # a NaN stays one
+        z = ops.mx_linear(x, codes, scales, None, n, k, epilogue=epilogue, out_dtype=torch.bfloat16)
+        assert torch.equal(z.isnan(), y.isnan())
 
 
 def test_linear_leading_dimensions_strides_empty(cuda_device):
