@@ -903,7 +903,7 @@ Tensor mx_grad_input(const Tensor& dy, const Tensor& codes, const Tensor& scales
   const c10::cuda::CUDAGuard guard(dy.device());
   int64_t n = dy.size(-1);
   const Mx w = mx_operand(codes, scales, &n, k, DIMQ_MX_FP4, "weight");
-  const Tensor g = dy.contiguous();
+  const Tensor g = aligned16(dy);
   Tensor dx = at::empty(out_shape(dy, k), dy.options().dtype(dt).memory_format(at::MemoryFormat::Contiguous));
   const int64_t m = mx_rows(dy, n);
   int64_t need = 0;
@@ -927,7 +927,7 @@ std::pair<OptTensor, OptTensor> mx_grad_weight(const Tensor& dy, const Tensor& c
   int64_t m = mx_rows(dy, n);
   same_device(codes, dy, "activation codes");
   const Mx x = mx_operand(codes, scales, &m, k, format, "activation");
-  const Tensor g = dy.contiguous();
+  const Tensor g = aligned16(dy);
   OptTensor dw, db;
   const auto opt = dy.options().memory_format(at::MemoryFormat::Contiguous);
   if (dw_dtype.has_value()) dw = at::empty({n, k}, opt.dtype(*dw_dtype));
@@ -947,7 +947,7 @@ Tensor mx_column_sum(const Tensor& dy, at::ScalarType dt, int* launches) {
   const int dyd = dtype_code(dy, "grad");
   if (dy.dim() == 0 || dy.size(-1) <= 0) fail("mx_column_sum expects a last dimension of out_features");
   const c10::cuda::CUDAGuard guard(dy.device());
-  const Tensor g = dy.contiguous();
+  const Tensor g = aligned16(dy);
   const int64_t n = dy.size(-1), m = mx_rows(dy, n);
   Tensor db = at::empty({n}, dy.options().dtype(dt).memory_format(at::MemoryFormat::Contiguous));
   int64_t need = 0;

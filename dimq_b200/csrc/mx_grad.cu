@@ -1,101 +1,393 @@
-// The gradients of the microscaled linear layer.
+// The gradients of the microscaled linear layer, straight through its rounding: dx = dy w^ and dw = dy^T x~.
 //
-// One plain kernel for both: 64 x 64 tiles of the result, 16 of the reduction at a time decoded to fp32 in shared
-// memory, 4 x 4 results a thread.
-#include "mx_common.cuh"
+// Both reduce over the slow axis of the coded operand (w^ [N][K] over n, x~ [M][K] over m), along which the block scales
+// change, so the scales cannot be left to the block-scaled tensor cores.  A coded value is exact in bf16 (at most eight
+// significant bits, bf16 has fp32's range), so the coded matrix is decoded once to scratch and multiplied by dy on the
+// 16-bit tensor cores, fp32 sums.  Nothing is transposed: TMA brings boxes of 64 columns (the decoded matrix is written
+// in panels of 64 columns, so that one copy brings all of a tile's), and the operand descriptors say that the columns are contiguous ("MN major") - w^ and x~ always, dy for dw.
+//
+// dy enters exactly: bf16 as it is, fp16 and fp32 as the sum of two or three bf16 terms, each the leading eight bits of
+// what the ones before left (24 bits in all; an infinity or a NaN is its own first term).  The terms are passes over the
+// same reduction, smallest first.
+//
+// The tensor cores cut their sums to fp32 instead of rounding them: the error grows with the number of steps.  Where the
+// result is fp32 it is therefore added up in registers, 512 values of the reduction at a time.
+//
+// Tile: 128 rows x BN columns of the result, ring stages of 64 of the reduction, two accumulators in tensor memory.
+// Warps 0-2 fetch, taking the stages in turn, warp 3 issues the MMAs, warps 4-11 are the epilogue, two to a lane quarter.
+#include "mx_tile.cuh"
 
 namespace dimq {
+int mx_decode_panels(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out, cudaStream_t st);
+
 namespace {
 
 using namespace mx;
 
-struct Coded {   // a microscaled matrix [rows][cols]
-  const uint8_t* codes;
-  const uint8_t* scales;
-  int64_t blocks, tiles;
-  int fp4;
-  __device__ float at(int64_t r, int64_t k) const {
-    const float f = scale_of(scales[scale_offset(r, k >> 5, tiles)]);
-    float v[8];
-    if (fp4) {
-      decode_fp4(codes[r * blocks * 16 + (k >> 1)] >> (4 * (k & 1)), v);
-      return v[0] * f;
-    }
-    return static_cast<float>(static_cast<int8_t>(codes[r * blocks * 32 + k])) * 0.015625f * f;
-  }
-};
-Coded coded(const void* codes, const uint8_t* scales, int64_t cols, int format) {
-  return {static_cast<const uint8_t*>(codes), scales, blocks_of(cols), block_tiles(cols), format == DIMQ_MX_FP4};
-}
+constexpr int kProducers = 3;
+constexpr int kThreads = (kProducers + 1 + kEpiWarps) * 32;
+constexpr int kMaxStages = 8;
+constexpr int kDepth = 64;                       // reduction per stage
+constexpr uint32_t kABytes = 128 * kDepth * 2;
+constexpr int kSegStages = 8;
 
-struct Dense {
-  const void* p;
-  int dtype;
-  int64_t cols;
-  __device__ float at(int64_t r, int64_t k) const { return load_as_float(p, dtype, r * cols + k); }
+struct GradMaps {
+  CUtensorMap a, b, y;
 };
 
-// c[r][j] = sum_t A(r, t) B(t, j); AT / BT: the operand is stored with its axes exchanged
-template <typename A, bool AT, typename B, bool BT>
-__global__ void __launch_bounds__(256)
-mx_plain_kernel(A a, B b, int64_t R, int64_t J, int64_t T, const void* bias, int bias_dtype, const void* residual, void* c,
-                int c_dtype, int epilogue) {
-  __shared__ float sa[16][65], sb[16][65];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, j0 = static_cast<int64_t>(blockIdx.x) * 64;
-  float acc[4][4] = {};
-  for (int64_t t0 = 0; t0 < T; t0 += 16) {
-    for (int i = threadIdx.x; i < 1024; i += 256) {
-      const int t = AT ? i >> 6 : i & 15, r = AT ? i & 63 : i >> 4;
-      const bool in = r0 + r < R && t0 + t < T;
-      sa[t][r] = in ? (AT ? a.at(t0 + t, r0 + r) : a.at(r0 + r, t0 + t)) : 0.0f;
-      const int tb = BT ? i & 15 : i >> 6, j = BT ? i >> 4 : i & 63;
-      const bool inb = j0 + j < J && t0 + tb < T;
-      sb[tb][j] = inb ? (BT ? b.at(j0 + j, t0 + tb) : b.at(t0 + tb, j0 + j)) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < 16; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[t][ty + 16 * i], sb[t][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = r0 + ty + 16 * i, k = j0 + tx + 16 * j;
-      if (r >= R || k >= J) continue;
-      float v = acc[i][j];
-      if (bias != nullptr) v += load_as_float(bias, bias_dtype, k);
-      v = finish_value(v, epilogue, residual != nullptr, residual != nullptr ? load_as_float(residual, c_dtype, r * J + k) : 0.0f);
-      store_from_float(c, c_dtype, r * J + k, v);
-    }
+struct GradParams {
+  Out out;
+  int depth_blocks;        // 64-blocks of the reduction, per term
+  int terms;
+  int stages, n_tiles, m_tiles;
+  int a_cols;              // dy's rows are the reduction (dw): its boxes are 64 columns x 64 rows
+};
+
+struct GradHeader {
+  uint64_t full[kMaxStages], empty[kMaxStages], d_full[2], d_empty[2];
+  uint32_t tmem_base;
+  volatile uint32_t abort_flag;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Columns contiguous: pieces of 64 columns x 8 rows of the reduction (1024 bytes, 128-byte swizzle), the next eight rows
+// 1024 bytes on, the next 64 columns a whole box (64 rows) on.
+__device__ __forceinline__ uint64_t columns_desc(uint32_t smem) {
+  return static_cast<uint64_t>((smem & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kDepth * 128 >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
 }
 
+template <int BN, int ES, bool SEG>
+__global__ void __launch_bounds__(kThreads, 1)
+mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
+  constexpr uint32_t kStageBytes = kABytes + BN * kDepth * 2;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t n_st = static_cast<uint32_t>(p.stages);
+  GradHeader* hdr = reinterpret_cast<GradHeader*>(smem + n_st * kStageBytes);
+  unsigned char* staging = reinterpret_cast<unsigned char*>(hdr) + kHeaderBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int steps = p.depth_blocks * p.terms, tiles = p.n_tiles * p.m_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), kEpiWarps); }
+    hdr->abort_flag = 0u;
+    fence_barrier_init();
+    prefetch_tensormap(&maps.a);
+    prefetch_tensormap(&maps.b);
+    if (p.out.tma) prefetch_tensormap(&maps.y);
+  }
+  if (warp == kProducers) {
+    tmem_alloc(smem_u32(&hdr->tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = hdr->tmem_base;
+  volatile uint32_t* abort_flag = &hdr->abort_flag;
+  wait_for_inputs();
+
+  if (warp < kProducers) {
+    // no more producers than stages, as in the forward product
+    const uint32_t turns = n_st < kProducers ? n_st : kProducers;
+    uint32_t stage = 0, phase = 0, turn = 0, issued = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int n_blk = t % p.n_tiles, m_blk = t / p.n_tiles;
+      for (int term = p.terms - 1; term >= 0 && ok; --term) {
+        for (int kb = 0; kb < p.depth_blocks; ++kb) {
+          if (turn == static_cast<uint32_t>(warp)) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase ^ 1u, abort_flag, 0x3100u | stage))) { ok = false; break; }
+            const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * kStageBytes);
+            if (elect_one()) {
+              mbar_arrive_expect_tx(full, kStageBytes);
+              if (p.a_cols) {
+                tma_load_3d(dst, &maps.a, full, m_blk * 128, kb * kDepth, term);
+                tma_load_3d(dst + kABytes / 2, &maps.a, full, m_blk * 128 + 64, kb * kDepth, term);
+              } else {
+                tma_load_3d(dst, &maps.a, full, kb * kDepth, m_blk * 128, term);
+              }
+              tma_load_3d(dst + kABytes, &maps.b, full, 0, kb * kDepth, n_blk * (BN / 64));
+            }
+            __syncwarp();
+          }
+          ++issued;
+          if (++turn == turns) turn = 0;
+          if (++stage == n_st) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+    if (!ok && lane == 0) {   // gave up: bounded wait for the copies in flight
+      const uint32_t n_back = issued < n_st ? issued : n_st;
+      uint32_t s = stage, ph = phase;
+      for (uint32_t i = 0; i < n_back; ++i) {
+        if (s == 0) { s = n_st - 1; ph ^= 1u; } else { --s; }
+        for (uint32_t it = 0; it < kSpinLimit; ++it)
+          if (mbar_try_wait(smem_u32(&hdr->full[s]), ph)) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == kProducers) {
+    uint32_t stage = 0, phase = 0, buf = 0, bph = 0;
+    bool ok = true;
+    const uint32_t idesc = make_idesc_f16(1, 1, 128, BN) | (p.a_cols ? 1u << 15 : 0u) | (1u << 16);
+    const uint64_t a_step = p.a_cols ? 2048 >> 4 : 32 >> 4;   // 16 of the reduction
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int seg0 = 0; seg0 < steps && ok; seg0 += SEG ? kSegStages : steps) {
+        const int seg1 = SEG && seg0 + kSegStages < steps ? seg0 + kSegStages : steps;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_empty[buf]), bph ^ 1u, abort_flag, 0x3200u | buf))) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d = tmem + buf * 256;
+        for (int s = seg0; s < seg1; ++s) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->full[stage]), phase, abort_flag, 0x3300u | stage))) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t at = smem_u32(smem + stage * kStageBytes);
+          const uint64_t a0 = p.a_cols ? columns_desc(at) : make_smem_desc_sw128(at), b0 = columns_desc(at + kABytes);
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < kDepth / 16; ++j)
+              mma_bf16(d, a0 + a_step * j, b0 + static_cast<uint64_t>((2048 >> 4) * j), idesc, (s > seg0 || j) ? 1u : 0u);
+            mma_commit(smem_u32(&hdr->empty[stage]));
+          }
+          __syncwarp();
+          if (++stage == n_st) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        if (elect_one()) mma_commit(smem_u32(&hdr->d_full[buf]));
+        __syncwarp();
+        if (++buf == 2) { buf = 0; bph ^= 1u; }
+      }
+    }
+  } else {
+    const int ew = warp - kProducers - 1;
+    const int quarter = warp & 3, sub = ew >> 2;
+    unsigned char* stage = staging + ew * (ES == 2 && p.out.tma ? 2048 : 4096);
+    constexpr int kMine = BN / 64;
+    uint32_t buf = 0, bph = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int64_t n_first = static_cast<int64_t>(t % p.n_tiles) * BN, row0 = static_cast<int64_t>(t / p.n_tiles) * 128 + quarter * 32;
+      const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+      float sum[SEG ? kMine : 1][32];
+      for (int seg0 = 0; seg0 < steps; seg0 += SEG ? kSegStages : steps) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x3500u | buf))) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const uint32_t col = tmem + lanes + buf * 256 + (sub + 2 * i) * 32;
+          if constexpr (SEG) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t r[16];
+              tmem_ld16(col + 16 * h, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) sum[i][16 * h + j] = (seg0 == 0 ? 0.0f : sum[i][16 * h + j]) + __uint_as_float(r[j]);
+            }
+          } else {
+            uint32_t r[32];
+            tmem_ld32(col, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[0][j] = __uint_as_float(r[j]);
+          }
+          if (i == kMine - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&hdr->d_empty[buf]));
+          }
+          __syncwarp();
+          if constexpr (!SEG) {
+            const int64_t n0 = n_first + (sub + 2 * i) * 32;
+            if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[0], p.out, &maps.y, stage, 0.0f, row0, n0, lane);
+          }
+        }
+        if (++buf == 2) { buf = 0; bph ^= 1u; }
+      }
+      if (!ok) break;
+      if constexpr (SEG) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int64_t n0 = n_first + (sub + 2 * i) * 32;
+          if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[i], p.out, &maps.y, stage, 0.0f, row0, n0, lane);
+        }
+      }
+    }
+    __syncwarp();
+    if (elect_one()) tma_store_wait_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kProducers) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// dy [rows][cols] -> TERMS bf16 matrices [rows][pitch] whose sum it is; zeros behind the last column
+template <typename T, int TERMS>
 __global__ void __launch_bounds__(256)
-mx_column_sum_kernel(Dense a, int64_t rows, void* out, int out_dtype) {
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
-  __shared__ float part[8][32];
-  float s = 0.0f;
-  if (j < a.cols)
-    for (int64_t r = threadIdx.x >> 5; r < rows; r += 8) s += a.at(r, j);
+mx_terms_kernel(const T* __restrict__ dy, int64_t rows, int64_t cols, int64_t pitch, uint16_t* __restrict__ out) {
+  const int64_t per_row = pitch / 8;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < rows * per_row; u += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = u / per_row, c = (u - row * per_row) * 8;
+    uint32_t w[TERMS][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = c + i < cols ? to_float<T>(dy[row * cols + c + i]) : 0.0f;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) {
+        uint32_t h = __float_as_uint(v) >> 16;       // cut, not rounded: a large value stays finite
+        if (v != v) h = 0x7FFFu;
+        const float f = __uint_as_float(h << 16);
+        v = (h & 0x7F80u) == 0x7F80u ? 0.0f : v - f;
+        if (i & 1) w[t][i >> 1] |= h << 16;
+        else w[t][i >> 1] = h;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t)
+      *reinterpret_cast<uint4*>(out + (t * rows + row) * pitch + c) = make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
+  }
+}
+
+// Column sums: a block takes 64 columns of a run of rows, its eight warps the rows in turn; the runs' sums are added by
+// a second kernel, in order.
+constexpr int kSumRows = 512;
+__global__ void __launch_bounds__(256)
+mx_column_sum_kernel(const void* __restrict__ dy, int dtype, int64_t rows, int64_t cols, float* __restrict__ partial, void* __restrict__ out,
+                     int out_dtype) {
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 31) * 2;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
+  __shared__ float2 part[8][32];
+  float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+  for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
+    if (j < cols) s.x += load_as_float(dy, dtype, r * cols + j);
+    if (j + 1 < cols) s.y += load_as_float(dy, dtype, r * cols + j + 1);
+  }
   part[threadIdx.x >> 5][threadIdx.x & 31] = s;
   __syncthreads();
-  if (threadIdx.x < 32 && j < a.cols) {
-    for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
-    store_from_float(out, out_dtype, j, s);
+  if (threadIdx.x >= 32) return;
+  for (int i = 1; i < 8; ++i) { s.x += part[i][threadIdx.x].x; s.y += part[i][threadIdx.x].y; }
+  if (gridDim.y > 1) {
+    float* p = partial + blockIdx.y * cols;
+    if (j < cols) p[j] = s.x;
+    if (j + 1 < cols) p[j + 1] = s.y;
+  } else {
+    if (j < cols) store_from_float(out, out_dtype, j, s.x);
+    if (j + 1 < cols) store_from_float(out, out_dtype, j + 1, s.y);
   }
 }
+__global__ void __launch_bounds__(256)
+mx_column_sum_finish_kernel(const float* __restrict__ partial, int64_t runs, int64_t cols, void* __restrict__ out, int out_dtype) {
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (j >= cols) return;
+  float s = 0.0f;
+  for (int64_t r = 0; r < runs; ++r) s += partial[r * cols + j];
+  store_from_float(out, out_dtype, j, s);
+}
 
-template <typename A, bool AT, typename B, bool BT>
-int plain(A a, B b, int64_t R, int64_t J, int64_t T, const void* bias, int bias_dtype, const void* residual, void* c, int c_dtype,
-          int epilogue, cudaStream_t st) {
-  const int64_t gx = (J + 63) / 64, gy = (R + 63) / 64;
-  if (gx > 0x7FFFFFFF || gy > 65535) return DIMQ_ERR_TOO_LARGE;
-  mx_plain_kernel<A, AT, B, BT><<<dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), 256, 0, st>>>(
-      a, b, R, J, T, bias, bias_dtype, residual, c, c_dtype, epilogue);
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+int terms_of(int dtype) { return dtype == DIMQ_BF16 ? 1 : dtype == DIMQ_F16 ? 2 : 3; }
+bool as_it_is(int dtype, int64_t cols) { return dtype == DIMQ_BF16 && cols % 8 == 0; }
+int64_t decoded_bytes(int64_t rows, int64_t K) { return up(rows * up(K, 64) * 2, 256); }
+int64_t terms_bytes(int dtype, int64_t M, int64_t N) { return as_it_is(dtype, N) ? 0 : up(terms_of(dtype) * M * up(N, 8) * 2, 256); }
+int64_t partial_bytes(int64_t M, int64_t N) { return M > kSumRows ? up((M + kSumRows - 1) / kSumRows * N * 4, 256) : 0; }
+
+// dy as the tensor cores take it: itself, or its terms in scratch
+int split_terms(const void* dy, int dtype, int64_t M, int64_t N, void* scratch, const void** a, int64_t* pitch, cudaStream_t st) {
+  *a = dy;
+  *pitch = N;
+  if (as_it_is(dtype, N)) return DIMQ_OK;
+  *a = scratch;
+  *pitch = up(N, 8);
+  const int64_t units = M * (*pitch / 8), blocks = (units + 255) / 256;
+  const unsigned grid = static_cast<unsigned>(blocks < kNumSMs * 16 ? blocks : kNumSMs * 16);
+  uint16_t* out = static_cast<uint16_t*>(scratch);
+  if (dtype == DIMQ_F32) mx_terms_kernel<float, 3><<<grid, 256, 0, st>>>(static_cast<const float*>(dy), M, N, *pitch, out);
+  else if (dtype == DIMQ_F16) mx_terms_kernel<__half, 2><<<grid, 256, 0, st>>>(static_cast<const __half*>(dy), M, N, *pitch, out);
+  else mx_terms_kernel<__nv_bfloat16, 1><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(dy), M, N, *pitch, out);
   return launch_status();
+}
+
+template <int BN, int ES, bool SEG>
+int launch_grad(GradMaps& maps, GradParams& p, cudaStream_t st) {
+  constexpr size_t kStageBytes = kABytes + BN * kDepth * 2;
+  const size_t fixed = 1024 + kHeaderBytes + kEpiWarps * (ES == 2 && p.out.tma ? 2048 : 4096);
+  p.stages = static_cast<int>((kSmemMax - fixed) / kStageBytes);
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  auto kern = mx_grad_kernel<BN, ES, SEG>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  const unsigned grid = static_cast<unsigned>(tiles < kNumSMs ? tiles : kNumSMs);
+  e = launch_dependent(kern, grid, kThreads, fixed + p.stages * kStageBytes, st, 1, maps, p);
+  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+}
+
+// out [R][K] = A * decoded, A = dy (reduction over its columns) or dy^T (over its rows, a_cols); `depth` values reduced
+int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms, bool a_cols, const void* decoded, int64_t depth, int64_t K,
+                 const Out& out, cudaStream_t st) {
+  GradMaps maps;
+  GradParams p = {};
+  p.out = out;
+  p.terms = terms;
+  p.a_cols = a_cols;
+  p.depth_blocks = static_cast<int>((depth + kDepth - 1) / kDepth);
+  // tile width: the fewest waves, weighed by what a stage of that width costs
+  const int width[3] = {256, 128, 64};
+  const double cost[3] = {750.0, 520.0, 430.0};
+  int bn = 256;
+  double least = 0.0;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t t = row_tiles(out.rows) * ((K + width[i] - 1) / width[i]);
+    const double c = static_cast<double>((t + kNumSMs - 1) / kNumSMs) * cost[i];
+    if (i == 0 || c < least) { least = c; bn = width[i]; }
+  }
+  const int64_t n_tiles = (K + bn - 1) / bn, m_tiles = row_tiles(out.rows);
+  if (n_tiles * m_tiles > 0x7FFFFFFF - kNumSMs || static_cast<int64_t>(p.depth_blocks) * terms > 0x7FFFFFFF - 64) return DIMQ_ERR_TOO_LARGE;
+  p.n_tiles = static_cast<int>(n_tiles);
+  p.m_tiles = static_cast<int>(m_tiles);
+  const CUtensorMapDataType bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const cuuint64_t adims[3] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(M), static_cast<cuuint64_t>(terms)};
+  const cuuint64_t astr[2] = {static_cast<cuuint64_t>(pitch) * 2, static_cast<cuuint64_t>(pitch) * 2 * static_cast<cuuint64_t>(M)};
+  const cuuint32_t abox[3] = {64, a_cols ? 64u : 128u, 1};
+  const cuuint64_t bdims[3] = {64, static_cast<cuuint64_t>(depth), static_cast<cuuint64_t>(up(K, 64) / 64)};
+  const cuuint64_t bstr[2] = {128, static_cast<cuuint64_t>(depth) * 128};
+  const cuuint32_t bbox[3] = {64, kDepth, static_cast<cuuint32_t>(bn / 64)};
+  if (!encode_map(&maps.a, bf16, 3, dy, adims, astr, abox, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_map(&maps.b, bf16, 3, decoded, bdims, bstr, bbox, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      (out.tma && !encode_out(&maps.y, out)))
+    return DIMQ_ERR_DRIVER;
+  const bool wide = out.dtype == DIMQ_F32, seg = wide && p.depth_blocks * terms > kSegStages;
+#define DIMQ_MX_GRAD(ES, SEG)                                        \
+  return bn == 256 ? launch_grad<256, ES, SEG>(maps, p, st)          \
+         : bn == 128 ? launch_grad<128, ES, SEG>(maps, p, st) : launch_grad<64, ES, SEG>(maps, p, st)
+  if (seg) DIMQ_MX_GRAD(4, true);
+  if (wide) DIMQ_MX_GRAD(4, false);
+  DIMQ_MX_GRAD(2, false);
+#undef DIMQ_MX_GRAD
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K) {
@@ -104,25 +396,54 @@ int check_sizes(int64_t M, int64_t N, int64_t K) {
   return DIMQ_OK;
 }
 
+int64_t grad_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+  return decoded_bytes(M > N ? M : N, K) + terms_bytes(dtype, M, N) + partial_bytes(M, N);
+}
+
+int clear(void* p, int dtype, int64_t n, cudaStream_t st) {   // a sum over no rows
+  const cudaError_t e = cudaMemsetAsync(p, 0, static_cast<size_t>(n) * dtype_size(dtype), st);
+  return e == cudaSuccess ? DIMQ_OK : static_cast<int>(e);
+}
+
 }  // namespace
+
+int read_mx_grad_status(uint32_t* status) { return tc::read_and_clear_device_status(status); }
+
 }  // namespace dimq
 
 using namespace dimq;
 
+extern "C" int dimq_mx_grad_workspace_bytes(int dy_dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes) {
+  if (bytes == nullptr) return DIMQ_ERR_NULL_POINTER;
+  *bytes = 0;
+  if (!valid_dtype(dy_dtype)) return DIMQ_ERR_BAD_DTYPE;
+  const int rc = check_sizes(M, N, K);
+  if (rc != DIMQ_OK) return rc;
+  *bytes = grad_bytes(dy_dtype, M, N, K);
+  return DIMQ_OK;
+}
+
 extern "C" int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, void* dx,
                                   int dx_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                                   void* stream) {
-  const int rc = check_sizes(M, N, K);
+  int rc = check_sizes(M, N, K);
   if (rc != DIMQ_OK) return rc;
   if (!valid_dtype(dy_dtype) || !valid_dtype(dx_dtype)) return DIMQ_ERR_BAD_DTYPE;
   if (M == 0) return DIMQ_OK;
   if (dy == nullptr || w_codes == nullptr || w_scales == nullptr || dx == nullptr) return DIMQ_ERR_NULL_POINTER;
-  if (!aligned(w_codes, 16) || !aligned(w_scales, 16) || !aligned(workspace, 16)) return DIMQ_ERR_ALIGNMENT;
-  int64_t need = 0;
-  dimq_mx_grad_workspace_bytes(dy_dtype, M, N, K, &need);
-  if (workspace == nullptr || workspace_bytes < need) return DIMQ_ERR_SCRATCH_TOO_SMALL;
-  return plain<Dense, false, Coded, false>(Dense{dy, dy_dtype, N}, coded(w_codes, w_scales, K, DIMQ_MX_FP4), M, K, N, nullptr, 0,
-                                           nullptr, dx, dx_dtype, DIMQ_EPI_NONE, static_cast<cudaStream_t>(stream));
+  if (!aligned(dy, 16) || !aligned(w_codes, 16) || !aligned(w_scales, 16) || !aligned(workspace, 256)) return DIMQ_ERR_ALIGNMENT;
+  if (workspace == nullptr || workspace_bytes < grad_bytes(dy_dtype, M, N, K)) return DIMQ_ERR_SCRATCH_TOO_SMALL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned char* decoded = static_cast<unsigned char*>(workspace);
+  const void* a;
+  int64_t pitch;
+  rc = split_terms(dy, dy_dtype, M, N, decoded + decoded_bytes(M > N ? M : N, K), &a, &pitch, st);
+  if (rc != DIMQ_OK) return rc;
+  rc = mx_decode_panels(w_codes, w_scales, DIMQ_MX_FP4, N, K, decoded, st);
+  if (rc != DIMQ_OK) return rc;
+  mx::Out out = {dx, nullptr, nullptr, M, K, 0, dx_dtype, DIMQ_EPI_NONE, 0};
+  out.tma = mx::out_by_map(out);
+  return grad_product(a, M, N, pitch, terms_of(dy_dtype), false, decoded, N, K, out, st);
 }
 
 extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_codes, const uint8_t* x_scales, int format, void* dw,
@@ -133,24 +454,35 @@ extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_c
   if (!mx::valid_format(format)) return DIMQ_ERR_BAD_BITS;
   if (!valid_dtype(dy_dtype) || (dw != nullptr && !valid_dtype(dw_dtype)) || (db != nullptr && !valid_dtype(db_dtype))) return DIMQ_ERR_BAD_DTYPE;
   if ((dw == nullptr && db == nullptr) || (M > 0 && (dy == nullptr || (dw != nullptr && (x_codes == nullptr || x_scales == nullptr))))) return DIMQ_ERR_NULL_POINTER;
-  if (!aligned(x_codes, 16) || !aligned(x_scales, 16) || !aligned(workspace, 16)) return DIMQ_ERR_ALIGNMENT;
-  int64_t need = 0;
-  dimq_mx_grad_workspace_bytes(dy_dtype, M, N, K, &need);
-  if (workspace == nullptr || workspace_bytes < need) return DIMQ_ERR_SCRATCH_TOO_SMALL;
+  if (!aligned(dy, 16) || !aligned(x_codes, 16) || !aligned(x_scales, 16) || !aligned(workspace, 256)) return DIMQ_ERR_ALIGNMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dw != nullptr)
-    rc = plain<Dense, true, Coded, false>(Dense{dy, dy_dtype, N}, coded(x_codes, x_scales, K, format), N, K, M, nullptr, 0, nullptr, dw,
-                                        dw_dtype, DIMQ_EPI_NONE, st);
-  if (rc != DIMQ_OK || db == nullptr) return rc;
-  mx_column_sum_kernel<<<static_cast<unsigned>((N + 31) / 32), 256, 0, st>>>(Dense{dy, dy_dtype, N}, M, db, db_dtype);
-  return launch_status();
-}
-
-extern "C" int dimq_mx_grad_workspace_bytes(int dy_dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes) {
-  if (bytes == nullptr) return DIMQ_ERR_NULL_POINTER;
-  *bytes = 0;
-  if (!valid_dtype(dy_dtype)) return DIMQ_ERR_BAD_DTYPE;
-  const int rc = check_sizes(M, N, K);
-  if (rc == DIMQ_OK) *bytes = 16;
-  return rc;
+  if (M == 0) {
+    if (dw != nullptr) rc = clear(dw, dw_dtype, N * K, st);
+    if (rc == DIMQ_OK && db != nullptr) rc = clear(db, db_dtype, N, st);
+    return rc;
+  }
+  if (workspace == nullptr || workspace_bytes < grad_bytes(dy_dtype, M, N, K)) return DIMQ_ERR_SCRATCH_TOO_SMALL;
+  unsigned char* decoded = static_cast<unsigned char*>(workspace);
+  unsigned char* terms = decoded + decoded_bytes(M > N ? M : N, K);
+  float* partial = reinterpret_cast<float*>(terms + terms_bytes(dy_dtype, M, N));
+  if (db != nullptr) {
+    const int64_t runs = (M + kSumRows - 1) / kSumRows, gx = (N + 63) / 64;
+    if (runs > 65535) return DIMQ_ERR_TOO_LARGE;
+    mx_column_sum_kernel<<<dim3(static_cast<unsigned>(gx), static_cast<unsigned>(runs)), 256, 0, st>>>(dy, dy_dtype, M, N, partial, db, db_dtype);
+    if ((rc = launch_status()) != DIMQ_OK) return rc;
+    if (runs > 1) {
+      mx_column_sum_finish_kernel<<<static_cast<unsigned>((N + 255) / 256), 256, 0, st>>>(partial, runs, N, db, db_dtype);
+      if ((rc = launch_status()) != DIMQ_OK) return rc;
+    }
+  }
+  if (dw == nullptr) return DIMQ_OK;
+  const void* a;
+  int64_t pitch;
+  rc = split_terms(dy, dy_dtype, M, N, terms, &a, &pitch, st);
+  if (rc != DIMQ_OK) return rc;
+  rc = mx_decode_panels(x_codes, x_scales, format, M, K, decoded, st);
+  if (rc != DIMQ_OK) return rc;
+  mx::Out out = {dw, nullptr, nullptr, N, K, 0, dw_dtype, DIMQ_EPI_NONE, 0};
+  out.tma = mx::out_by_map(out);
+  return grad_product(a, M, N, pitch, terms_of(dy_dtype), true, decoded, M, K, out, st);
 }

@@ -110,11 +110,12 @@ mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t 
   }
 }
 
-// out rows of `pitch` values: the `cols` of the row, then zeros up to `fill`
-template <typename T, bool VEC, bool FP4>
+// Without PANELS out is [rows][cols].  With them it is [columns / 64][rows][64], zeros behind the last column: what TMA
+// takes as boxes of 64 columns.  fill: columns written (cols, or the panels' 64s).
+template <typename T, bool VEC, bool FP4, bool PANELS>
 __global__ void __launch_bounds__(kThreads)
 mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
-                     int64_t spans, T* __restrict__ out, int64_t pitch, int64_t fill) {
+                     int64_t spans, T* __restrict__ out, int64_t fill) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t group = static_cast<int64_t>(blockIdx.x) / spans, span = static_cast<int64_t>(blockIdx.x) - group * spans;
   const int64_t tile = group >> 2;
@@ -150,7 +151,7 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
     T o[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = from_float<T>(k + i < cols ? v[i] * f : 0.0f);
-    T* dst = out + row * pitch + k;
+    T* dst = PANELS ? out + ((k >> 6) * rows + row) * 64 + (k & 63) : out + row * cols + k;
     if (VEC && k + 8 <= fill) {
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
@@ -194,19 +195,19 @@ int quantize_as(const void* x, int64_t rows, int64_t cols, void* c4, uint8_t* s4
   return launch_status();
 }
 
-template <typename T>
-int dequantize_as(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out, int64_t pitch,
-                  int64_t fill, cudaStream_t st) {
+template <typename T, bool PANELS>
+int dequantize_as(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out, cudaStream_t st) {
   int64_t spans;
   unsigned grid;
+  const int64_t fill = PANELS ? (cols + 63) / 64 * 64 : cols;
   const int rc = grid_of(rows, fill, &spans, &grid);
   if (rc != DIMQ_OK) return rc;
   const uint8_t* in = static_cast<const uint8_t*>(codes);
   T* o = static_cast<T*>(out);
-  const bool vec = aligned(out, 16) && (pitch * static_cast<int64_t>(sizeof(T))) % 16 == 0;
-#define DIMQ_MX_D(V, F) mx_dequantize_kernel<T, V, F><<<grid, kThreads, 0, st>>>(in, scales, rows, cols, spans, o, pitch, fill)
-  if (format == DIMQ_MX_FP4) { if (vec) DIMQ_MX_D(true, true); else DIMQ_MX_D(false, true); }
-  else { if (vec) DIMQ_MX_D(true, false); else DIMQ_MX_D(false, false); }
+  const bool vec = PANELS || (aligned(out, 16) && (cols * static_cast<int64_t>(sizeof(T))) % 16 == 0);
+#define DIMQ_MX_D(V, F) mx_dequantize_kernel<T, V, F, PANELS><<<grid, kThreads, 0, st>>>(in, scales, rows, cols, spans, o, fill)
+  if (format == DIMQ_MX_FP4) { if (vec) DIMQ_MX_D(true, true); else DIMQ_MX_D(PANELS, true); }
+  else { if (vec) DIMQ_MX_D(true, false); else DIMQ_MX_D(PANELS, false); }
 #undef DIMQ_MX_D
   return launch_status();
 }
@@ -222,10 +223,15 @@ int mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, void* c4
 }
 
 int mx_dequantize(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out, int out_dtype,
-                  int64_t pitch, int64_t fill, cudaStream_t st) {
-  if (out_dtype == DIMQ_F32) return dequantize_as<float>(codes, scales, format, rows, cols, out, pitch, fill, st);
-  if (out_dtype == DIMQ_F16) return dequantize_as<__half>(codes, scales, format, rows, cols, out, pitch, fill, st);
-  return dequantize_as<__nv_bfloat16>(codes, scales, format, rows, cols, out, pitch, fill, st);
+                  cudaStream_t st) {
+  if (out_dtype == DIMQ_F32) return dequantize_as<float, false>(codes, scales, format, rows, cols, out, st);
+  if (out_dtype == DIMQ_F16) return dequantize_as<__half, false>(codes, scales, format, rows, cols, out, st);
+  return dequantize_as<__nv_bfloat16, false>(codes, scales, format, rows, cols, out, st);
+}
+
+// the same as bf16 panels [ceil(cols / 64)][rows][64], 16-byte aligned
+int mx_decode_panels(const void* codes, const uint8_t* scales, int format, int64_t rows, int64_t cols, void* out, cudaStream_t st) {
+  return dequantize_as<__nv_bfloat16, true>(codes, scales, format, rows, cols, out, st);
 }
 
 }  // namespace dimq
@@ -280,5 +286,5 @@ extern "C" int dimq_mx_dequantize(const void* codes, const uint8_t* scales, int 
   if (rows == 0) return DIMQ_OK;
   if (codes == nullptr || scales == nullptr || out == nullptr) return DIMQ_ERR_NULL_POINTER;
   if (!aligned(codes, 16) || !aligned(scales, 16)) return DIMQ_ERR_ALIGNMENT;
-  return mx_dequantize(codes, scales, format, rows, cols, out, out_dtype, cols, cols, static_cast<cudaStream_t>(stream));
+  return mx_dequantize(codes, scales, format, rows, cols, out, out_dtype, static_cast<cudaStream_t>(stream));
 }

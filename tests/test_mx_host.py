@@ -34,7 +34,7 @@ def test_sizes(lib):
 
 
 def test_argument_errors_are_reported_without_a_gpu(lib):
-    null, one, odd = C.c_void_p(0), C.c_void_p(16), C.c_void_p(24)
+    null, one, odd = C.c_void_p(0), C.c_void_p(256), C.c_void_p(24)
     i = C.c_int64
     assert lib.dimq_mx_quantize(one, 7, i(1), i(32), 4, one, one, null) == -3
     assert lib.dimq_mx_quantize(one, 0, i(1), i(32), 3, one, one, null) == -4
