@@ -67,6 +67,7 @@ int launch_linear_prepack(const uint8_t* packed, int bits, int64_t N, int64_t K,
 int read_dense_status(uint32_t* status);
 int read_mx_status(uint32_t* status);
 int read_mx_grad_status(uint32_t* status);
+int read_mx_small_status(uint32_t* status);
 int launch_bounded_wait_selftest(uint32_t polls, uint32_t* result, cudaStream_t st);
 }  // namespace dimq
 
@@ -124,7 +125,7 @@ extern "C" const char* dimq_status_string(int status) {
 
 extern "C" int dimq_last_device_status(uint32_t* status) {
   if (status == nullptr) return DIMQ_ERR_NULL_POINTER;
-  uint32_t tc = 0, ms = 0, dense = 0, rg = 0, mx = 0, mxg = 0;
+  uint32_t tc = 0, ms = 0, dense = 0, rg = 0, mx = 0, mxg = 0, mxs = 0;
   int rc = read_device_status(&tc);
   if (rc != DIMQ_OK) return rc;
   rc = read_ms_status(&ms);
@@ -137,7 +138,9 @@ extern "C" int dimq_last_device_status(uint32_t* status) {
   if (rc != DIMQ_OK) return rc;
   rc = read_mx_grad_status(&mxg);
   if (rc != DIMQ_OK) return rc;
-  *status = tc | ms | dense | rg | mx | mxg;
+  rc = read_mx_small_status(&mxs);
+  if (rc != DIMQ_OK) return rc;
+  *status = tc | ms | dense | rg | mx | mxg | mxs;
   return DIMQ_OK;
 }
 

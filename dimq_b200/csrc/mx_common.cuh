@@ -47,6 +47,46 @@ __device__ __forceinline__ uint32_t encode_fp4_pair(float lo, float hi) {
   asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
+template <typename T>
+struct Eight {   // eight consecutive values as they are loaded
+  uint4 q[sizeof(T) / 2];
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t k, int64_t cols, float (&v)[8]) {
+  constexpr int kPer = 16 / sizeof(T);   // values per 16 bytes; rows are whole 16-byte pieces where VEC
+  if (VEC) {
+    Eight<T> e;
+#pragma unroll
+    for (int i = 0; i < 8 / kPer; ++i) {
+      e.q[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (k + i * kPer < cols) e.q[i] = __ldg(reinterpret_cast<const uint4*>(row + k + i * kPer));
+    }
+    const T* p = reinterpret_cast<const T*>(&e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_float<T>(p[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < cols ? to_float<T>(row[k + i]) : 0.0f;
+  }
+}
+
+// bits of the largest |v| of a block that four neighbouring lanes hold, eight values each
+__device__ __forceinline__ uint32_t block_top(const float (&v)[8]) {
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  return max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+}
+// eight values of a block whose scale byte is b -> codes
+__device__ __forceinline__ uint32_t encode_fp4(const float (&v)[8], uint32_t b) {
+  const float f = inverse_scale(b);
+  uint32_t w = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= encode_fp4_pair(v[2 * i] * f, v[2 * i + 1] * f) << (8 * i);
+  return b == 255u ? 0u : w;
+}
 // eight e2m1 codes -> floats.  A code's three bits, moved to a half's lowest exponent bits and highest mantissa bit, are
 // its magnitude times 2^-14, subnormal code and all.
 __device__ __forceinline__ void decode_fp4(uint32_t w, float (&v)[8]) {

@@ -14,6 +14,9 @@
 namespace dimq {
 int mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, void* c4, uint8_t* s4, void* c8, uint8_t* s8,
                 cudaStream_t st);
+bool mx_small_takes(int64_t M, int64_t N, int64_t K);
+int mx_small(const void* x, int x_dtype, const uint8_t* wc, const uint8_t* ws, const void* bias, int bias_dtype, const void* residual,
+             void* y, int y_dtype, int64_t M, int64_t N, int64_t K, int epilogue, cudaStream_t st);
 
 namespace {
 
@@ -43,29 +46,6 @@ struct GemmHeader {
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
-
-// scale tile (32 rows x 16 bytes) -> 4 columns, the same in all four lane quarters
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-}
-// rows of 16 bytes, eight to a 128-byte group, no swizzle
-__device__ __forceinline__ uint64_t scale_desc(uint32_t smem) {
-  return static_cast<uint64_t>((smem & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 16) |
-         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
-}
-__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
-}
-// e2m1 times e2m1 with e8m0 scales; `half`: which two of the four scale bytes of a column belong to this step
-__host__ __device__ constexpr uint32_t mxf4_idesc(int m, int n, int half) {
-  return (static_cast<uint32_t>(2 * half) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
-         (static_cast<uint32_t>(m >> 7) << 27) | (static_cast<uint32_t>(2 * half) << 29);
-}
 
 template <int BN>
 struct Shape {
@@ -272,13 +252,6 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
   }
 }
 
-bool code_map(CUtensorMap* m, const void* codes, int64_t rows, int64_t K, int box_rows) {   // bytes, 128 of them a box row
-  const cuuint64_t pitch = static_cast<cuuint64_t>(codes_pitch(K, DIMQ_MX_FP4));
-  const cuuint64_t dims[2] = {pitch, static_cast<cuuint64_t>(rows)};
-  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
-  return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, &pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 template <int BN, int ES, bool SEG>
 int launch_gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& out, int64_t K, cudaStream_t st) {
   using S = Shape<BN>;
@@ -353,7 +326,7 @@ extern "C" int dimq_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, i
   *bytes = 0;
   const int rc = check_sizes(M, N, K);
   if (rc != DIMQ_OK) return rc;
-  if (!coded) *bytes = codes_room(M, K) + mx::scales_bytes(M, K);
+  if (!coded && !mx_small_takes(M, N, K)) *bytes = codes_room(M, K) + mx::scales_bytes(M, K);
   return DIMQ_OK;
 }
 
@@ -371,6 +344,8 @@ extern "C" int dimq_mx_linear(const void* x, int x_dtype, const uint8_t* x_scale
     return DIMQ_ERR_ALIGNMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint8_t *xc = static_cast<const uint8_t*>(x), *xs = x_scales;
+  if (x_scales == nullptr && mx_small_takes(M, N, K))
+    return mx_small(x, x_dtype, w_codes, w_scales, bias, bias_dtype, residual, y, y_dtype, M, N, K, epilogue, st);
   if (x_scales == nullptr) {
     if (workspace == nullptr || workspace_bytes < codes_room(M, K) + mx::scales_bytes(M, K)) return DIMQ_ERR_SCRATCH_TOO_SMALL;
     uint8_t* c = static_cast<uint8_t*>(workspace);

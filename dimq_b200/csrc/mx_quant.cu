@@ -14,30 +14,6 @@ constexpr int kThreads = 256;
 constexpr int kSpan = 256;        // features a warp takes at a time
 constexpr int kRowsPerBlock = 8;  // rows r of one row tile, each with its three rows 32 further
 
-template <typename T>
-struct Eight {   // eight consecutive values as they are loaded
-  uint4 q[sizeof(T) / 2];
-};
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t k, int64_t cols, float (&v)[8]) {
-  constexpr int kPer = 16 / sizeof(T);   // values per 16 bytes; rows are whole 16-byte pieces where VEC
-  if (VEC) {
-    Eight<T> e;
-#pragma unroll
-    for (int i = 0; i < 8 / kPer; ++i) {
-      e.q[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (k + i * kPer < cols) e.q[i] = __ldg(reinterpret_cast<const uint4*>(row + k + i * kPer));
-    }
-    const T* p = reinterpret_cast<const T*>(&e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float<T>(p[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < cols ? to_float<T>(row[k + i]) : 0.0f;
-  }
-}
-
 // the four bytes of a half warp's blocks in one word, known to all its lanes
 __device__ __forceinline__ uint32_t gather_bytes(uint32_t b, int lane) {
   uint32_t w = b << (8 * ((lane >> 2) & 3));
@@ -71,20 +47,12 @@ mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t 
   uint32_t s4[4], s8[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    uint32_t top = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[q][i]) & 0x7FFFFFFFu);
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    const uint32_t top = block_top(v[q]);
     const int64_t row = row0 + 32 * q;
     const bool write = row < rows && k < blocks * kBlock;
     if (C4) {
       const uint32_t b = scale_byte(top, 2);
-      const float f = inverse_scale(b);
-      uint32_t w = 0u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w |= encode_fp4_pair(v[q][2 * i] * f, v[q][2 * i + 1] * f) << (8 * i);
-      if (b == 255u) w = 0u;
+      const uint32_t w = encode_fp4(v[q], b);
       if (write) *reinterpret_cast<uint32_t*>(codes4 + row * blocks * 16 + (k >> 1)) = w;
       s4[q] = gather_bytes(b, lane);
     }

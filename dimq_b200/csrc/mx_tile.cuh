@@ -78,6 +78,29 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
 }
 
+// scale tile (32 rows x 16 bytes) -> 4 columns, the same in all four lane quarters
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// rows of 16 bytes, eight to a 128-byte group, no swizzle
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem) {
+  return static_cast<uint64_t>((smem & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// e2m1 times e2m1 with e8m0 scales; `half`: which two of the four scale bytes of a column belong to this step
+__device__ constexpr uint32_t mxf4_idesc(int m, int n, int half) {
+  return (static_cast<uint32_t>(2 * half) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(m >> 7) << 27) | (static_cast<uint32_t>(2 * half) << 29);
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -193,6 +216,14 @@ __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CU
 }
 
 #endif
+
+// codes of a 4-bit matrix, boxes of 128 bytes (256 values) x box_rows
+inline bool code_map(CUtensorMap* m, const void* codes, int64_t rows, int64_t K, int box_rows) {
+  const cuuint64_t pitch = static_cast<cuuint64_t>(codes_pitch(K, DIMQ_MX_FP4));
+  const cuuint64_t dims[2] = {pitch, static_cast<cuuint64_t>(rows)};
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+  return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, &pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
 
 inline bool out_by_map(const Out& o) {
   const int64_t es = o.dtype == DIMQ_F32 ? 4 : 2;
