@@ -2,8 +2,8 @@
 //
 // What bounds it is reading the weight, so the weight is the wide operand: a block takes 128 of its rows as the lanes of
 // the block-scaled MMA (kind::mxf4, see mx_gemm.cu) and the rows of x as its columns, and a cluster of blocks divides k.
-// Every block fires all its copies at once - codes and scales of its slice, up to 102 KB - and quantises its slice of x
-// while they come; then a few MMAs, and the cluster adds its partial sums over distributed shared memory, in rank order,
+// A block starts as many copies as its ring holds before it looks at x, and quantises its slice of x while they come; then
+// steps of 256 k go through the ring, and the cluster adds its partial sums over distributed shared memory, in rank order,
 // each block finishing a share of the rows.
 #include "mx_tile.cuh"
 
@@ -13,12 +13,15 @@ namespace {
 using namespace mx;
 
 constexpr int kThreads = 256;
-constexpr int kMostSteps = 6;                 // 256-k steps a block holds
+constexpr int kMostSteps = 16;                // 256-k steps of a block (their x is kept whole)
 constexpr int kMostSlices = 8;                // blocks of a cluster
-// Tensor-memory columns of a block, 32 of sums and 16 of scales per step, in powers of two.  A block that waits for columns
-// keeps its cluster waiting, and so the columns that its peers hold: the blocks that fit on an SM must never want more than
-// its 512.  So a block asks for at least as much shared memory (28.5 KB for every 64 columns) as makes that so for any mix.
-__host__ __device__ constexpr uint32_t columns_of(int room) { return room <= 2 ? 64u : 128u; }
+constexpr int kMostStages = 6;
+constexpr uint32_t kWeightBytes = 128 * 128 + 1024;   // a ring stage: the codes of 128 rows x 256 k, and their scales
+// Tensor-memory columns of a block: 32 of sums and 16 of scales per ring stage, a power of two.  A block that waits for
+// columns keeps its cluster waiting, and so the columns that its peers hold: the blocks that fit on an SM must never want
+// more than its 512.  So a block asks for at least as much shared memory (28.5 KB for every 64 columns) as makes that so
+// for any mix of such blocks.
+__host__ __device__ constexpr uint32_t columns_of(int stages) { return stages <= 2 ? 64u : 128u; }
 constexpr size_t kBytesPer64Columns = 28 * 1024 + 512;
 
 struct SmallParams {
@@ -27,11 +30,11 @@ struct SmallParams {
   Out out;                                    // rows = M, cols = N
   int64_t K;
   int k_tiles, steps, slices;                 // scale tiles along k, 256-k steps, blocks of a cluster
-  int room;                                   // steps a block has room for
+  int room, stages;                           // steps a block has room for x of, ring stages
 };
 
 struct SmallHeader {
-  uint64_t full, done;
+  uint64_t full[kMostStages], empty[kMostStages], done;
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -55,17 +58,13 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
 }
 
-// bytes of a 256-k step: 128 weight rows, their scales, NB rows of x, theirs
-constexpr uint32_t step_bytes(int nb) { return 128u * 128u + 1024u + static_cast<uint32_t>(nb) * 128u + 1024u; }
-
 template <int NB, typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  // [step: weight codes][step: weight scales][step: x codes][step: x scales][sums NB x 128][header], all by steps of room
-  unsigned char* s_sfa = smem + p.room * 16384;
-  unsigned char* s_x = s_sfa + p.room * 1024;
+  // [stage: weight codes, scales][step: x codes][step: x scales][sums NB x 128][header]
+  unsigned char* s_x = smem + p.stages * kWeightBytes;
   unsigned char* s_sfx = s_x + p.room * (NB * 128);
   float* s_sum = reinterpret_cast<float*>(s_sfx + p.room * 1024);
   SmallHeader* hdr = reinterpret_cast<SmallHeader*>(s_sum + NB * 128);
@@ -76,43 +75,53 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
   const int tiles_here = min(2 * n_steps, p.k_tiles - 2 * step0);
 
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(&hdr->full), 1);
+    for (int i = 0; i < kMostStages; ++i) { mbar_init(smem_u32(&hdr->full[i]), 1); mbar_init(smem_u32(&hdr->empty[i]), 1); }
     mbar_init(smem_u32(&hdr->done), 1);
     hdr->abort_flag = 0u;
     fence_barrier_init();
+    prefetch_tensormap(&codes);
   }
   __syncwarp();
+  const auto load_step = [&](int i, int stage) {   // one lane
+    const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * kWeightBytes);
+    const uint32_t sf = static_cast<uint32_t>(min(2, tiles_here - 2 * i)) * kTileBytes;
+    mbar_arrive_expect_tx(full, 16384u + sf);
+    tma_load_2d(dst, &codes, full, (step0 + i) * 128, row_tile * 128);
+    bulk_load(dst + 16384, p.sfa + (static_cast<int64_t>(row_tile) * p.k_tiles + 2 * (step0 + i)) * kTileBytes, sf, full);
+  };
+  wait_for_inputs();
   if (warp == 0) {
-    if (elect_one()) {      // the whole slice of the weight at once
-      const uint32_t full = smem_u32(&hdr->full);
-      mbar_arrive_expect_tx(full, static_cast<uint32_t>(n_steps) * 16384u + static_cast<uint32_t>(tiles_here) * kTileBytes);
-      for (int i = 0; i < n_steps; ++i) tma_load_2d(smem_u32(smem + i * 16384), &codes, full, (step0 + i) * 128, row_tile * 128);
-      bulk_load(smem_u32(s_sfa), p.sfa + (static_cast<int64_t>(row_tile) * p.k_tiles + 2 * step0) * kTileBytes,
-                static_cast<uint32_t>(tiles_here) * kTileBytes, full);
-    }
+    if (elect_one())
+      for (int i = 0; i < p.stages && i < n_steps; ++i) load_step(i, i);
     __syncwarp();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&hdr->tmem_base), columns_of(p.room));
+    tmem_alloc(smem_u32(&hdr->tmem_base), columns_of(p.stages));
     tmem_relinquish();
   }
 
-  // this slice of x: four lanes hold a block of 32, eight values each
+  // this slice of x: four lanes hold a block of 32, eight values each; kAhead blocks' loads in flight
   {
+    constexpr int kAhead = 4;
     const int blocks = tiles_here * 4, rows = static_cast<int>(p.out.rows);
     const int units = rows * blocks;
     const T* x = static_cast<const T*>(p.x);
-    for (int u0 = warp * 8; u0 < units; u0 += kThreads / 4) {
-      const int u = u0 + (lane >> 2);
-      const int r = min(u / blocks, rows - 1), b = u - (u / blocks) * blocks;
-      const int64_t k = static_cast<int64_t>(step0) * 256 + b * 32 + (lane & 3) * 8;
-      float v[8];
-      load8<T, VEC>(x + r * p.K, k, p.K, v);
-      const uint32_t byte = scale_byte(block_top(v), 2);
-      if (u < units) {
-        const int step = b >> 3, piece = b & 7;      // 16 bytes of codes: piece of the step's 128-byte row, swizzled
-        *reinterpret_cast<uint32_t*>(s_x + step * (NB * 128) + r * 128 + ((piece ^ (r & 7)) << 4) + (lane & 3) * 4) = encode_fp4(v, byte);
-        if ((lane & 3) == 0) s_sfx[step * 1024 + ((b >> 2) & 1) * kTileBytes + r * 16 + (b & 3)] = static_cast<uint8_t>(byte);
+    for (int u0 = warp * 8; u0 < units; u0 += kAhead * (kThreads / 4)) {
+      float v[kAhead][8];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int u = min(u0 + i * (kThreads / 4) + (lane >> 2), units - 1), r = u / blocks;
+        load8<T, VEC>(x + r * p.K, static_cast<int64_t>(step0) * 256 + (u - r * blocks) * 32 + (lane & 3) * 8, p.K, v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int u = u0 + i * (kThreads / 4) + (lane >> 2), r = u / blocks, b = u - r * blocks;
+        const uint32_t byte = scale_byte(block_top(v[i]), 2);
+        if (u < units) {
+          const int step = b >> 3, piece = b & 7;    // 16 bytes of codes: piece of the step's 128-byte row, swizzled
+          *reinterpret_cast<uint32_t*>(s_x + step * (NB * 128) + r * 128 + ((piece ^ (r & 7)) << 4) + (lane & 3) * 4) = encode_fp4(v[i], byte);
+          if ((lane & 3) == 0) s_sfx[step * 1024 + ((b >> 2) & 1) * kTileBytes + r * 16 + (b & 3)] = static_cast<uint8_t>(byte);
+        }
       }
     }
   }
@@ -120,29 +129,48 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  let_dependents_start();       // every block of this grid runs by now and has its columns
   const uint32_t tmem = hdr->tmem_base;
   bool ok = true;
   if (warp == 0) {
-    ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->full), 0u, &hdr->abort_flag, 0x4100u));
-    if (ok) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < n_steps; ++i) {
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->full[stage]), phase, &hdr->abort_flag, 0x4100u | stage))) { ok = false; break; }
       if (elect_one()) {
-        const uint64_t sfa0 = scale_desc(smem_u32(s_sfa)), sfx0 = scale_desc(smem_u32(s_sfx));
-        for (int t = 0; t < tiles_here; ++t) {
-          copy_scales(tmem + 32 + 8 * t, sfa0 + static_cast<uint64_t>(t * (kTileBytes >> 4)));
-          copy_scales(tmem + 36 + 8 * t, sfx0 + static_cast<uint64_t>(t * (kTileBytes >> 4)));
-        }
-        for (int t = 0; t < tiles_here; ++t) {
-          const uint64_t a = make_smem_desc_sw128(smem_u32(smem + (t >> 1) * 16384)) + static_cast<uint64_t>(4 * (t & 1));
-          const uint64_t b = make_smem_desc_sw128(smem_u32(s_x + (t >> 1) * (NB * 128))) + static_cast<uint64_t>(4 * (t & 1));
+        const uint32_t w = smem_u32(smem + stage * kWeightBytes), sfa = tmem + 32 + 16 * stage, sfx = sfa + 8;
+        const uint64_t sfa0 = scale_desc(w + 16384), sfx0 = scale_desc(smem_u32(s_sfx + i * 1024));
+        const uint64_t a0 = make_smem_desc_sw128(w), b0 = make_smem_desc_sw128(smem_u32(s_x + i * (NB * 128)));
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            mma_mxf4(tmem, a + 2 * j, b + 2 * j, mxf4_idesc(128, NB, j), tmem + 32 + 8 * t, tmem + 36 + 8 * t, (t | j) ? 1u : 0u);
+        for (int t = 0; t < 2; ++t) {
+          if (2 * i + t < tiles_here) {
+            copy_scales(sfa + 4 * t, sfa0 + static_cast<uint64_t>(t * (kTileBytes >> 4)));
+            copy_scales(sfx + 4 * t, sfx0 + static_cast<uint64_t>(t * (kTileBytes >> 4)));
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              mma_mxf4(tmem, a0 + 4 * t + 2 * j, b0 + 4 * t + 2 * j, mxf4_idesc(128, NB, j), sfa + 4 * t, sfx + 4 * t, (i | t | j) ? 1u : 0u);
+          }
         }
-        mma_commit(smem_u32(&hdr->done));
+        mma_commit(smem_u32(&hdr->empty[stage]));
+        if (i == n_steps - 1) mma_commit(smem_u32(&hdr->done));
       }
-    } else {                // gave up: bounded wait for the copies in flight
-      for (uint32_t it = 0; it < kSpinLimit; ++it)
-        if (mbar_try_wait(smem_u32(&hdr->full), 0u)) break;
+      __syncwarp();
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+    }
+  } else if (warp == 1) {       // the ring's later rounds
+    int stage = 0;
+    uint32_t phase = 0;
+    int i = p.stages;
+    for (; i < n_steps; ++i) {
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase, &hdr->abort_flag, 0x4300u | stage))) { ok = false; break; }
+      if (elect_one()) load_step(i, stage);
+      __syncwarp();
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+    }
+    if (!ok) {                  // gave up: bounded wait for the copies in flight, the last of every stage
+      for (int j = i - p.stages < 0 ? 0 : i - p.stages; j < i; ++j)
+        for (uint32_t it = 0; it < kSpinLimit; ++it)
+          if (mbar_try_wait(smem_u32(&hdr->full[j % p.stages]), static_cast<uint32_t>(j / p.stages) & 1u)) break;
     }
     __syncwarp();
   }
@@ -200,31 +228,27 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, columns_of(p.room));
+    tmem_dealloc(tmem, columns_of(p.stages));
   }
 }
 
 template <int NB, typename T>
-int launch_small(const CUtensorMap& codes, const SmallParams& p, bool vec, int64_t row_blocks, cudaStream_t st) {
-  size_t smem = 1024 + p.room * step_bytes(NB) + NB * 512 + 64;
-  const size_t least = columns_of(p.room) / 64 * kBytesPer64Columns;
+int launch_small(const CUtensorMap& codes, SmallParams p, bool vec, int64_t row_blocks, cudaStream_t st) {
+  const size_t fixed = 1024 + p.room * (NB * 128 + 1024) + NB * 512 + sizeof(SmallHeader) + 64;
+  // a ring as deep as leaves room for the blocks of this grid side by side (three to an SM at most)
+  const int64_t blocks = row_blocks * p.slices, per_sm = blocks <= kNumSMs ? 1 : blocks <= 2 * kNumSMs ? 2 : 3;
+  const int64_t free = static_cast<int64_t>(kSmemMax / per_sm) - 1024 - static_cast<int64_t>(fixed);
+  p.stages = static_cast<int>(free / static_cast<int64_t>(kWeightBytes));
+  if (p.stages > kMostStages) p.stages = kMostStages;
+  if (p.stages > p.room) p.stages = p.room;
+  if (p.stages < 2) p.stages = p.room < 2 ? 1 : 2;
+  size_t smem = fixed + p.stages * kWeightBytes;
+  const size_t least = columns_of(p.stages) / 64 * kBytesPer64Columns;
   if (smem < least) smem = least;
   auto kern = vec ? mx_small_kernel<NB, T, true> : mx_small_kernel<NB, T, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
   if (e != cudaSuccess) return static_cast<int>(e);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(row_blocks * p.slices));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(p.slices);
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, codes, p);
+  e = launch_dependent(kern, static_cast<unsigned>(blocks), kThreads, smem, st, p.slices, codes, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
@@ -250,8 +274,11 @@ int mx_small(const void* x, int x_dtype, const uint8_t* wc, const uint8_t* ws, c
   p.k_tiles = static_cast<int>(block_tiles(K));
   p.steps = (p.k_tiles + 1) / 2;
   const int64_t row_blocks = row_tiles(N);
+  // as many blocks as run side by side, three to an SM
   int slices = 1;
-  while (slices < kMostSlices && 2 * slices <= p.steps && (row_blocks * slices < 2 * kNumSMs || (p.steps + slices - 1) / slices > kMostSteps)) slices *= 2;
+  while (slices < kMostSlices && 2 * slices <= p.steps &&
+         (row_blocks * slices * 2 <= 3 * kNumSMs || (p.steps + slices - 1) / slices > kMostSteps))
+    slices *= 2;
   p.slices = slices;
   p.room = (p.steps + slices - 1) / slices;
   CUtensorMap codes;

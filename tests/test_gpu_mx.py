@@ -136,7 +136,7 @@ def _check_linear(y, x4, w4, bias, epilogue, residual, out_dtype):
 
 LINEAR = [(1, 1, 1), (1, 32, 8), (3, 33, 7), (2, 100, 128), (8, 256, 130), (16, 1000, 129), (17, 1024, 64), (1, 4096, 256), (5, 8320, 128),
           (33, 520, 257), (64, 2050, 100), (128, 128, 128), (130, 300, 257), (197, 768, 96), (300, 1001, 515), (257, 512, 640),
-          (2500, 330, 2568), (1300, 4420, 2600)]
+          (16, 16500, 130), (5, 32768, 40), (3, 33000, 40), (2500, 330, 2568), (1300, 4420, 2600)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
