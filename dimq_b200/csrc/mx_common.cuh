@@ -41,75 +41,156 @@ __device__ __forceinline__ float inverse_scale(uint32_t b) {
   return __uint_as_float(b >= 254u ? 0x00400000u : (254u - b) << 23);
 }
 
-// two floats -> two e2m1 codes, `lo` in the low half; nearest even, saturating at 6
-__device__ __forceinline__ uint32_t encode_fp4_pair(float lo, float hi) {
-  uint32_t d;
-  asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
+// packed pairs of fp32
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+  uint64_t d, x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(b));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
 }
-template <typename T>
-struct Eight {   // eight consecutive values as they are loaded
-  uint4 q[sizeof(T) / 2];
-};
+__device__ __forceinline__ float2 add2(float2 a, float b) {
+  uint64_t d, x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(b));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t k, int64_t cols, float (&v)[8]) {
-  constexpr int kPer = 16 / sizeof(T);   // values per 16 bytes; rows are whole 16-byte pieces where VEC
-  if (VEC) {
-    Eight<T> e;
+// Eight consecutive values of a row as they are stored: what a lane holds of a block, four lanes to a block.
+template <typename T>
+struct Eight {
+  uint32_t w[2 * sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> no_values() {
+  Eight<T> e;
 #pragma unroll
-    for (int i = 0; i < 8 / kPer; ++i) {
-      e.q[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (k + i * kPer < cols) e.q[i] = __ldg(reinterpret_cast<const uint4*>(row + k + i * kPer));
-    }
-    const T* p = reinterpret_cast<const T*>(&e);
+  for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) e.w[i] = 0u;
+  return e;
+}
+// rows of whole 16-byte pieces
+template <typename T>
+__device__ __forceinline__ Eight<T> load_pieces(const T* __restrict__ row, int64_t k, int64_t cols) {
+  constexpr int kPer = 16 / sizeof(T);
+  Eight<T> e = no_values<T>();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float<T>(p[i]);
-  } else {
+  for (int i = 0; i < 8 / kPer; ++i)
+    if (k + i * kPer < cols) *reinterpret_cast<uint4*>(&e.w[4 * i]) = __ldg(reinterpret_cast<const uint4*>(row + k + i * kPer));
+  return e;
+}
+// any row: the warp reads neighbours (32 values at a time) and the values change hands in shared memory, `swap` 256 of
+// them; k0 is the first of the warp's 256.
+template <typename T>
+__device__ __forceinline__ void load_neighbours(const T* __restrict__ row, int64_t k0, int64_t cols, int lane, T (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < cols ? to_float<T>(row[k + i]) : 0.0f;
+  for (int i = 0; i < 8; ++i) {
+    const int64_t k = k0 + 32 * i + lane;
+    v[i] = k < cols ? row[k] : from_float<T>(0.0f);
   }
 }
+template <typename T>
+__device__ __forceinline__ Eight<T> change_hands(const T (&v)[8], T* swap, int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) swap[32 * i + lane] = v[i];
+  __syncwarp();
+  Eight<T> e;
+  const uint4* from = reinterpret_cast<const uint4*>(swap + 8 * lane);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) *reinterpret_cast<uint4*>(&e.w[4 * i]) = from[i];
+  return e;
+}
 
-// bits of the largest |v| of a block that four neighbouring lanes hold, eight values each
-__device__ __forceinline__ uint32_t block_top(const float (&v)[8]) {
+__device__ __forceinline__ float2 pair_of(const Eight<float>& e, int i) {
+  return make_float2(__uint_as_float(e.w[2 * i]), __uint_as_float(e.w[2 * i + 1]));
+}
+__device__ __forceinline__ float2 pair_of(const Eight<__half>& e, int i) { return __half22float2(*reinterpret_cast<const __half2*>(&e.w[i])); }
+__device__ __forceinline__ float2 pair_of(const Eight<__nv_bfloat16>& e, int i) {
+  return make_float2(__uint_as_float(e.w[i] << 16), __uint_as_float(e.w[i] & 0xFFFF0000u));
+}
+
+// bits (as fp32) of the largest |v| of a block; among bits without the sign a NaN is larger than an infinity, and that
+// larger than any number, in every type
+__device__ __forceinline__ uint32_t block_top(const Eight<float>& e) {
   uint32_t top = 0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < 8; ++i) top = max(top, e.w[i] & 0x7FFFFFFFu);
   top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
   return max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
 }
-// eight values of a block whose scale byte is b -> codes
-__device__ __forceinline__ uint32_t encode_fp4(const float (&v)[8], uint32_t b) {
+__device__ __forceinline__ uint32_t top_of_pairs(const uint32_t (&w)[4]) {
+  uint32_t top = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+  top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+  return max(top & 0xFFFFu, top >> 16);
+}
+__device__ __forceinline__ uint32_t block_top(const Eight<__nv_bfloat16>& e) { return top_of_pairs(e.w) << 16; }
+__device__ __forceinline__ uint32_t block_top(const Eight<__half>& e) {
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(top_of_pairs(e.w)))));
+}
+
+// eight values of a block whose scale byte is b -> e2m1 codes, nearest even, saturating at 6
+template <typename T>
+__device__ __forceinline__ uint32_t encode_fp4(const Eight<T>& e, uint32_t b) {
   const float f = inverse_scale(b);
-  uint32_t w = 0u;
+  float2 v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w |= encode_fp4_pair(v[2 * i] * f, v[2 * i + 1] * f) << (8 * i);
-  return b == 255u ? 0u : w;
+  for (int i = 0; i < 4; ++i) v[i] = mul2(pair_of(e, i), f);
+  uint32_t d;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(d) : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
+  return b == 255u ? 0u : d;
 }
-// eight e2m1 codes -> floats.  A code's three bits, moved to a half's lowest exponent bits and highest mantissa bit, are
-// its magnitude times 2^-14, subnormal code and all.
-__device__ __forceinline__ void decode_fp4(uint32_t w, float (&v)[8]) {
+// ... -> multiples of 1/64.  Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low byte.
+template <typename T>
+__device__ __forceinline__ uint2 encode_int8(const Eight<T>& e, uint32_t b) {
+  const float f = inverse_scale(b);
+  uint32_t c[8];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const uint32_t c = (w >> (4 * i)) & 0xFFu;
-    const uint32_t h = ((c & 0x7u) << 9) | ((c & 0x8u) << 12) | ((c & 0x70u) << 21) | ((c & 0x80u) << 24);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    v[i] = f.x * 16384.0f;
-    v[i + 1] = f.y * 16384.0f;
+  for (int i = 0; i < 4; ++i) {
+    float2 v = mul2(mul2(pair_of(e, i), f), 64.0f);
+    v = add2(make_float2(fminf(fmaxf(v.x, -127.0f), 127.0f), fminf(fmaxf(v.y, -127.0f), 127.0f)), 12582912.0f);
+    c[2 * i] = __float_as_uint(v.x);
+    c[2 * i + 1] = __float_as_uint(v.y);
   }
+  uint2 d;
+  d.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  d.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+  return b == 255u ? make_uint2(0u, 0u) : d;
 }
-__device__ __forceinline__ void decode_int8(uint2 w, float (&v)[8]) {
+
+// eight e2m1 codes -> their values times f
+__device__ __forceinline__ void decode_fp4(uint32_t w, float f, float2 (&v)[4]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t word = i < 4 ? w.x : w.y;
-    v[i] = static_cast<float>(static_cast<int8_t>(word >> (8 * (i & 3)))) * 0.015625f;
+  for (int i = 0; i < 4; ++i) v[i] = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h[i])), f);
+}
+// eight 8-bit codes -> their values times f.  A byte with its sign bit turned, under the exponent of 2^23, is 2^23 + 128 + code.
+__device__ __forceinline__ void decode_int8(uint2 w, float f, float2 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t word = (i < 2 ? w.x : w.y) ^ 0x80808080u;
+    const float2 c = make_float2(__uint_as_float(__byte_perm(word, 0x4B000000u, i & 1 ? 0x7542 : 0x7540)),
+                                 __uint_as_float(__byte_perm(word, 0x4B000000u, i & 1 ? 0x7543 : 0x7541)));
+    v[i] = mul2(mul2(add2(c, -8388736.0f), 0.015625f), f);
   }
 }
 
-__host__ __device__ __forceinline__ int64_t scale_offset(int64_t row, int64_t block, int64_t tiles) {
-  return ((row >> 7) * tiles + (block >> 2)) * kTileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
-}
+// programmatic dependents of this grid may start; what it writes is theirs after their own wait
+__device__ __forceinline__ void let_dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 }  // namespace mx
 }  // namespace dimq

@@ -2,7 +2,8 @@
 // lanes hold a block, eight values each, its largest magnitude takes two shuffles, and the rest is conversions.
 //
 // A warp takes the same 256 features of the rows r, r + 32, r + 64 and r + 96 of a row tile: four loads of 16 bytes a
-// lane in flight (fp32: eight), and the scale bytes of the four rows are the 16 that lie together in the tile.
+// lane in flight (fp32: eight), and the scale bytes of the four rows are the 16 that lie together in the tile.  Rows that
+// do not start on 16 bytes are read and written 32 neighbours at a time and change hands in shared memory.
 #include "mx_common.cuh"
 
 namespace dimq {
@@ -27,6 +28,7 @@ template <typename T, bool VEC, bool C4, bool C8>
 __global__ void __launch_bounds__(kThreads)
 mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t spans, uint8_t* __restrict__ codes4,
                    uint8_t* __restrict__ scales4, uint8_t* __restrict__ codes8, uint8_t* __restrict__ scales8) {
+  __shared__ __align__(16) unsigned char swap[VEC ? 16 : 8 * kSpan * sizeof(T)];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t group = static_cast<int64_t>(blockIdx.x) / spans, span = static_cast<int64_t>(blockIdx.x) - group * spans;
   const int64_t tile = group >> 2;
@@ -34,39 +36,34 @@ mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t 
   const int64_t row0 = tile * 128 + r;
   const int64_t k = span * kSpan + lane * 8;
   const int64_t blocks = blocks_of(cols), tiles = block_tiles(cols);
-  float v[4][8];
+  Eight<T> e[4];
+  let_dependents_start();
+  if constexpr (VEC) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (row0 + 32 * q < rows) {
-      load8<T, VEC>(x + (row0 + 32 * q) * cols, k, cols, v[q]);
-    } else {
+    for (int q = 0; q < 4; ++q) e[q] = row0 + 32 * q < rows ? load_pieces<T>(x + (row0 + 32 * q) * cols, k, cols) : no_values<T>();
+  } else {
+    T v[4][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[q][i] = 0.0f;
-    }
+    for (int q = 0; q < 4; ++q)
+      load_neighbours<T>(x + (row0 + 32 * q) * cols, span * kSpan, row0 + 32 * q < rows ? cols : 0, lane, v[q]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) e[q] = change_hands<T>(v[q], reinterpret_cast<T*>(swap) + warp * kSpan, lane);
   }
   uint32_t s4[4], s8[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const uint32_t top = block_top(v[q]);
+    const uint32_t top = block_top(e[q]);
     const int64_t row = row0 + 32 * q;
     const bool write = row < rows && k < blocks * kBlock;
     if (C4) {
-      const uint32_t b = scale_byte(top, 2);
-      const uint32_t w = encode_fp4(v[q], b);
+      const uint32_t b = scale_byte(top, 2), w = encode_fp4(e[q], b);
       if (write) *reinterpret_cast<uint32_t*>(codes4 + row * blocks * 16 + (k >> 1)) = w;
       s4[q] = gather_bytes(b, lane);
     }
     if (C8) {
       const uint32_t b = scale_byte(top, 0);
-      const float f = inverse_scale(b);
-      uint32_t w[2] = {0u, 0u};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = __float2int_rn(fminf(fmaxf(v[q][i] * f * 64.0f, -127.0f), 127.0f));
-        w[i >> 2] |= (static_cast<uint32_t>(c) & 0xFFu) << (8 * (i & 3));
-      }
-      if (b == 255u) w[0] = w[1] = 0u;
-      if (write) *reinterpret_cast<uint2*>(codes8 + row * blocks * 32 + k) = make_uint2(w[0], w[1]);
+      const uint2 w = encode_int8(e[q], b);
+      if (write) *reinterpret_cast<uint2*>(codes8 + row * blocks * 32 + k) = w;
       s8[q] = gather_bytes(b, lane);
     }
   }
@@ -78,12 +75,37 @@ mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t 
   }
 }
 
+template <typename T>
+__device__ __forceinline__ Eight<T> pack_values(const float2 (&v)[4]);
+template <>
+__device__ __forceinline__ Eight<float> pack_values<float>(const float2 (&v)[4]) {
+  Eight<float> e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { e.w[2 * i] = __float_as_uint(v[i].x); e.w[2 * i + 1] = __float_as_uint(v[i].y); }
+  return e;
+}
+template <>
+__device__ __forceinline__ Eight<__half> pack_values<__half>(const float2 (&v)[4]) {
+  Eight<__half> e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(e.w[i]) : "f"(v[i].y), "f"(v[i].x));
+  return e;
+}
+template <>
+__device__ __forceinline__ Eight<__nv_bfloat16> pack_values<__nv_bfloat16>(const float2 (&v)[4]) {
+  Eight<__nv_bfloat16> e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(e.w[i]) : "f"(v[i].y), "f"(v[i].x));
+  return e;
+}
+
 // Without PANELS out is [rows][cols].  With them it is [columns / 64][rows][64], zeros behind the last column: what TMA
 // takes as boxes of 64 columns.  fill: columns written (cols, or the panels' 64s).
 template <typename T, bool VEC, bool FP4, bool PANELS>
 __global__ void __launch_bounds__(kThreads)
 mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
                      int64_t spans, T* __restrict__ out, int64_t fill) {
+  __shared__ __align__(16) unsigned char swap[VEC ? 16 : 8 * kSpan * sizeof(T)];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t group = static_cast<int64_t>(blockIdx.x) / spans, span = static_cast<int64_t>(blockIdx.x) - group * spans;
   const int64_t tile = group >> 2;
@@ -93,7 +115,8 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
   const int64_t blocks = blocks_of(cols), tiles = block_tiles(cols);
   const bool have = k < blocks * kBlock;
   uint2 w[4];
-  uint32_t s[4] = {0u, 0u, 0u, 0u};
+  uint4 s = make_uint4(0u, 0u, 0u, 0u);
+  if (PANELS) let_dependents_start();
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     w[q] = make_uint2(0u, 0u);
@@ -103,36 +126,43 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
       else w[q] = __ldg(reinterpret_cast<const uint2*>(codes + row * blocks * 32 + k));
     }
   }
-  if (have) {
-    const uint4 t = __ldg(reinterpret_cast<const uint4*>(scales + (tile * tiles + span * 2 + (lane >> 4)) * kTileBytes + r * 16));
-    const int sh = 8 * ((lane >> 2) & 3);
-    s[0] = (t.x >> sh) & 0xFFu; s[1] = (t.y >> sh) & 0xFFu; s[2] = (t.z >> sh) & 0xFFu; s[3] = (t.w >> sh) & 0xFFu;
-  }
+  if (have) s = __ldg(reinterpret_cast<const uint4*>(scales + (tile * tiles + span * 2 + (lane >> 4)) * kTileBytes + r * 16));
+  const int sh = 8 * ((lane >> 2) & 3);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int64_t row = row0 + 32 * q;
-    if (row >= rows || k >= fill) continue;
-    float v[8];
-    if (FP4) decode_fp4(w[q].x, v);
-    else decode_int8(w[q], v);
-    const float f = scale_of(s[q]);
-    T o[8];
+    if (row >= rows) continue;        // the warp's
+    const float f = scale_of(((q == 0 ? s.x : q == 1 ? s.y : q == 2 ? s.z : s.w) >> sh) & 0xFFu);
+    float2 v[4];
+    if (FP4) decode_fp4(w[q].x, f, v);
+    else decode_int8(w[q], f, v);
+    if (PANELS && k + 8 > cols) {     // a block that reads as NaN ends where the row does
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = from_float<T>(k + i < cols ? v[i] * f : 0.0f);
-    T* dst = PANELS ? out + ((k >> 6) * rows + row) * 64 + (k & 63) : out + row * cols + k;
-    if (VEC && k + 8 <= fill) {
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
-        uint4 u;
-        T* p = reinterpret_cast<T*>(&u);
-#pragma unroll
-        for (int j = 0; j < 16 / static_cast<int>(sizeof(T)); ++j) p[j] = o[i * (16 / static_cast<int>(sizeof(T))) + j];
-        reinterpret_cast<uint4*>(dst)[i] = u;
+      for (int i = 0; i < 4; ++i) {
+        if (k + 2 * i >= cols) v[i].x = 0.0f;
+        if (k + 2 * i + 1 >= cols) v[i].y = 0.0f;
       }
-    } else {
+    }
+    const Eight<T> e = pack_values<T>(v);
+    if constexpr (VEC) {
+      T* dst = PANELS ? out + ((k >> 6) * rows + row) * 64 + (k & 63) : out + row * cols + k;
+      constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < fill) dst[i] = o[i];
+      for (int i = 0; i < 8 / kPer; ++i)
+        if (k + i * kPer < fill) *reinterpret_cast<uint4*>(dst + i * kPer) = make_uint4(e.w[4 * i], e.w[4 * i + 1], e.w[4 * i + 2], e.w[4 * i + 3]);
+    } else {                          // the values change hands, so that the warp stores neighbours
+      T* mine = reinterpret_cast<T*>(swap) + warp * kSpan;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+        reinterpret_cast<uint4*>(mine + 8 * lane)[i] = make_uint4(e.w[4 * i], e.w[4 * i + 1], e.w[4 * i + 2], e.w[4 * i + 3]);
+      __syncwarp();
+      T* dst = out + row * cols;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t c = span * kSpan + 32 * i + lane;
+        if (c < cols) dst[c] = mine[32 * i + lane];
+      }
     }
   }
 }

@@ -53,6 +53,15 @@ __device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
   return v;
 }
+template <typename T>
+__device__ __forceinline__ Eight<T> load_single(const T* __restrict__ row, int64_t k, int64_t cols) {
+  Eight<T> e = no_values<T>();
+  T* v = reinterpret_cast<T*>(e.w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < cols) v[i] = row[k + i];
+  return e;
+}
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
@@ -107,11 +116,12 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
     const int units = rows * blocks;
     const T* x = static_cast<const T*>(p.x);
     for (int u0 = warp * 8; u0 < units; u0 += kAhead * (kThreads / 4)) {
-      float v[kAhead][8];
+      Eight<T> v[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int u = min(u0 + i * (kThreads / 4) + (lane >> 2), units - 1), r = u / blocks;
-        load8<T, VEC>(x + r * p.K, static_cast<int64_t>(step0) * 256 + (u - r * blocks) * 32 + (lane & 3) * 8, p.K, v[i]);
+        const int64_t k = static_cast<int64_t>(step0) * 256 + (u - r * blocks) * 32 + (lane & 3) * 8;
+        v[i] = VEC ? load_pieces<T>(x + r * p.K, k, p.K) : load_single<T>(x + r * p.K, k, p.K);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
