@@ -5,6 +5,10 @@
 // brings codes (rows of 128 bytes = 256 values, 128-byte swizzle) and the 512-byte scale tiles that the format keeps,
 // tcgen05.cp moves a scale tile to tensor memory, and the accumulators go through bias, activation and residual to y.
 //
+// Large problems run on pairs of blocks (cta_group::2): 256 x 256 tiles, each block holding its 128 rows of x and half of
+// the tile's rows of w, so that a step moves 32 KB of codes into each shared memory instead of 48.  The first block of a
+// pair issues for both; the scales of w are in both tensor memories.
+//
 // Tile: 128 rows of x (one tensor-memory lane each) x BN rows of w.  A ring stage holds 256 k of both operands and their
 // scales; its scale columns in tensor memory belong to the stage too, so the commit that frees the stage frees them.
 // Warps 0-2 fetch (they take the stages in turn), warp 3 issues copies and MMAs, warps 4-11 are the epilogue: two to each
@@ -30,7 +34,7 @@ constexpr uint32_t kABytes = 128 * 128;
 constexpr int kSegStages = 8;                    // fp32 results: sums of 2048 k are added up in registers
 
 struct GemmMaps {
-  CUtensorMap a, b, y;
+  CUtensorMap a, b, y, sfa, sfb;   // scales: pairs only
 };
 
 struct GemmParams {
@@ -47,20 +51,21 @@ struct GemmHeader {
   volatile uint32_t abort_flag;
 };
 
-template <int BN>
+template <int BN, bool PAIR>
 struct Shape {
   static constexpr int kRowTiles = BN > 128 ? BN / 128 : 1;               // scale tiles of w a stage holds per k tile
-  static constexpr uint32_t kBBytes = BN * 128;
+  static constexpr uint32_t kBBytes = (PAIR ? BN / 2 : BN) * 128;
   static constexpr uint32_t kStageBytes = kABytes + kBBytes + 1024 + kRowTiles * 1024;
   static constexpr int kSfCols = 8 + 8 * kRowTiles;                      // tensor-memory columns of a stage's scales
   static constexpr int kBufs = BN > 128 ? 1 : 2;                         // accumulators
   static constexpr int kMost = (512 - kSfCol) / kSfCols < kMaxStages ? (512 - kSfCol) / kSfCols : kMaxStages;
 };
 
-template <int BN, int ES, bool SEG>
+// SEG: fp32 results of long sums, added up in registers (BN <= 128).  PAIR: BN = 256.
+template <int BN, int ES, bool SEG, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
-  using S = Shape<BN>;
+  using S = Shape<BN, PAIR>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t n_st = static_cast<uint32_t>(p.stages);
@@ -68,10 +73,13 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
   unsigned char* staging = reinterpret_cast<unsigned char*>(hdr) + kHeaderBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k_stages = (p.k_tiles + 1) / 2;
+  const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
+  const int tile0 = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int tile_step = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), kEpiWarps); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), PAIR ? 2 * kEpiWarps : kEpiWarps); }
     hdr->abort_flag = 0u;
     fence_barrier_init();
     prefetch_tensormap(&maps.a);
@@ -79,12 +87,13 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     if (p.out.tma) prefetch_tensormap(&maps.y);
   }
   if (warp == kProducers) {
-    tmem_alloc(smem_u32(&hdr->tmem_base), 512);
-    tmem_relinquish();
+    if constexpr (PAIR) tmem_alloc_pair(smem_u32(&hdr->tmem_base), 512);   // the same columns in both
+    else { tmem_alloc(smem_u32(&hdr->tmem_base), 512); tmem_relinquish(); }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if constexpr (PAIR) { cluster_arrive(); cluster_wait(); }   // the peer's barriers are there before anything signals them
   const uint32_t tmem = hdr->tmem_base;
   volatile uint32_t* abort_flag = &hdr->abort_flag;
   wait_for_inputs();
@@ -95,23 +104,34 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     const uint32_t turns = n_st < kProducers ? n_st : kProducers;
     uint32_t stage = 0, phase = 0, turn = 0, issued = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
-      const int n_blk = t % p.n_tiles, m_blk = t / p.n_tiles;
+    for (int t = tile0; t < p.tiles && ok; t += tile_step) {
+      const int n_blk = t % p.n_tiles, m_blk = (PAIR ? 2 : 1) * (t / p.n_tiles) + rank;
       for (int kb = 0; kb < k_stages; ++kb) {
         if (turn == static_cast<uint32_t>(warp)) {
           if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase ^ 1u, abort_flag, 0x2100u | stage))) { ok = false; break; }
           const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * S::kStageBytes);
-          const uint32_t sf_bytes = p.k_tiles - 2 * kb >= 2 ? 1024u : 512u;
-          const int rt0 = n_blk * BN / 128;
-          const int rts = S::kRowTiles < p.row_tiles_b - rt0 ? S::kRowTiles : p.row_tiles_b - rt0;
-          if (elect_one()) {
-            mbar_arrive_expect_tx(full, kABytes + S::kBBytes + sf_bytes * (1 + rts));
-            tma_load_2d(dst, &maps.a, full, kb * 128, m_blk * 128);
-            tma_load_2d(dst + kABytes, &maps.b, full, kb * 128, n_blk * BN);
-            const uint32_t sf = dst + kABytes + S::kBBytes;
-            bulk_load(sf, p.sfa + (static_cast<int64_t>(m_blk) * p.k_tiles + 2 * kb) * kTileBytes, sf_bytes, full);
-            for (int i = 0; i < rts; ++i)
-              bulk_load(sf + 1024 * (1 + i), p.sfb + (static_cast<int64_t>(rt0 + i) * p.k_tiles + 2 * kb) * kTileBytes, sf_bytes, full);
+          const uint32_t sf = dst + kABytes + S::kBBytes;
+          if constexpr (PAIR) {
+            if (elect_one()) {     // both blocks' bytes are counted in the first one's barrier
+              if (rank == 0) mbar_arrive_expect_tx(full, 2 * S::kStageBytes);
+              const uint32_t lead = map_to_cta(full, 0);
+              tma_load_2d_pair(dst, &maps.a, lead, kb * 128, m_blk * 128);
+              tma_load_2d_pair(dst + kABytes, &maps.b, lead, kb * 128, n_blk * BN + rank * (BN / 2));
+              tma_load_2d_pair(sf, &maps.sfa, lead, kb * 256, m_blk);
+              tma_load_2d_pair(sf + 1024, &maps.sfb, lead, kb * 256, n_blk * (BN / 128));
+            }
+          } else {
+            const uint32_t sf_bytes = p.k_tiles - 2 * kb >= 2 ? 1024u : 512u;
+            const int rt0 = n_blk * BN / 128;
+            const int rts = S::kRowTiles < p.row_tiles_b - rt0 ? S::kRowTiles : p.row_tiles_b - rt0;
+            if (elect_one()) {
+              mbar_arrive_expect_tx(full, kABytes + S::kBBytes + sf_bytes * (1 + rts));
+              tma_load_2d(dst, &maps.a, full, kb * 128, m_blk * 128);
+              tma_load_2d(dst + kABytes, &maps.b, full, kb * 128, n_blk * BN);
+              bulk_load(sf, p.sfa + (static_cast<int64_t>(m_blk) * p.k_tiles + 2 * kb) * kTileBytes, sf_bytes, full);
+              for (int i = 0; i < rts; ++i)
+                bulk_load(sf + 1024 * (1 + i), p.sfb + (static_cast<int64_t>(rt0 + i) * p.k_tiles + 2 * kb) * kTileBytes, sf_bytes, full);
+            }
           }
           __syncwarp();
         }
@@ -132,8 +152,8 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     __syncwarp();
   } else if (warp == kProducers) {
     uint32_t stage = 0, phase = 0, buf = 0, bph = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
+    bool ok = rank == 0;      // the first block of a pair issues for both
+    for (int t = tile0; t < p.tiles && ok; t += tile_step) {
       const int n0 = (t % p.n_tiles) * BN;
       for (int seg0 = 0; seg0 < k_stages && ok; seg0 += SEG ? kSegStages : k_stages) {
         const int seg1 = SEG && seg0 + kSegStages < k_stages ? seg0 + kSegStages : k_stages;
@@ -152,23 +172,24 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
               if (kt < kts) {   // a scale tile that is not there has no values either
-                copy_scales(sfa + 4 * kt, sf0 + static_cast<uint64_t>(kt * (kTileBytes >> 4)));
+                copy_scales<PAIR>(sfa + 4 * kt, sf0 + static_cast<uint64_t>(kt * (kTileBytes >> 4)));
 #pragma unroll
                 for (int i = 0; i < S::kRowTiles; ++i)
-                  copy_scales(sfb + (kt * S::kRowTiles + i) * 4, sf0 + static_cast<uint64_t>((1024 * (1 + i) + kt * kTileBytes) >> 4));
+                  copy_scales<PAIR>(sfb + (kt * S::kRowTiles + i) * 4, sf0 + static_cast<uint64_t>((1024 * (1 + i) + kt * kTileBytes) >> 4));
 #pragma unroll
                 for (int j = 0; j < 2; ++j)   // 64 k = 32 bytes inside the swizzled row
-                  mma_mxf4(d, a0 + static_cast<uint64_t>(4 * kt + 2 * j), b0 + static_cast<uint64_t>(4 * kt + 2 * j), mxf4_idesc(128, BN, j),
-                           sfa + 4 * kt, sfb + kt * S::kRowTiles * 4 + (BN == 64 && (n0 & 64) ? 2 : 0), (kb > seg0 || kt || j) ? 1u : 0u);
+                  mma_mxf4<PAIR>(d, a0 + static_cast<uint64_t>(4 * kt + 2 * j), b0 + static_cast<uint64_t>(4 * kt + 2 * j),
+                                 mxf4_idesc(PAIR ? 256 : 128, BN, j), sfa + 4 * kt,
+                                 sfb + kt * S::kRowTiles * 4 + (BN == 64 && (n0 & 64) ? 2 : 0), (kb > seg0 || kt || j) ? 1u : 0u);
               }
             }
-            mma_commit(smem_u32(&hdr->empty[stage]));
+            commit<PAIR>(smem_u32(&hdr->empty[stage]));
           }
           __syncwarp();
           if (++stage == n_st) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        if (elect_one()) mma_commit(smem_u32(&hdr->d_full[buf]));
+        if (elect_one()) commit<PAIR>(smem_u32(&hdr->d_full[buf]));
         __syncwarp();
         if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
       }
@@ -180,8 +201,9 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     constexpr int kChunks = BN / 32, kMine = kChunks / 2;
     uint32_t buf = 0, bph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < p.tiles && ok; t += gridDim.x) {
-      const int64_t n_first = static_cast<int64_t>(t % p.n_tiles) * BN, row0 = static_cast<int64_t>(t / p.n_tiles) * 128 + quarter * 32;
+    for (int t = tile0; t < p.tiles && ok; t += tile_step) {
+      const int64_t n_first = static_cast<int64_t>(t % p.n_tiles) * BN;
+      const int64_t row0 = (static_cast<int64_t>(PAIR ? 2 : 1) * (t / p.n_tiles) + rank) * 128 + quarter * 32;
       float bias[kMine];
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
@@ -189,11 +211,12 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
         bias[i] = p.out.bias != nullptr && n < p.out.cols ? load_as_float(p.out.bias, p.out.bias_dtype, n) : 0.0f;
       }
       const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-      if constexpr (SEG) {
-        float sum[kMine][32];
-        for (int seg0 = 0; seg0 < k_stages; seg0 += kSegStages) {
-          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf))) { ok = false; break; }
-          tc_fence_after();
+      float sum[kMine][32];
+      for (int seg0 = 0; seg0 < k_stages; seg0 += SEG ? kSegStages : k_stages) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf))) { ok = false; break; }
+        tc_fence_after();
+        // all of this warp's sums into registers: the accumulator is free before they are looked at
+        if constexpr (SEG) {
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {
             uint32_t r[32];
@@ -202,41 +225,25 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) sum[i][j] = seg0 == 0 ? __uint_as_float(r[j]) : sum[i][j] + __uint_as_float(r[j]);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&hdr->d_empty[buf]));
-          __syncwarp();
-          if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
-        }
-        if (!ok) break;
+        } else {
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int64_t n0 = n_first + (sub + 2 * i) * 32;
-          if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[i], p.out, &maps.y, stage, bias[i], row0, n0, lane);
-        }
-      } else {
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf))) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          uint32_t r[32];
-          tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, r);
+          for (int i = 0; i < kMine; ++i) tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, reinterpret_cast<uint32_t(&)[32]>(sum[i]));
           tmem_ld_wait();
-          if (i == kMine - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&hdr->d_empty[buf]));
-          }
-          __syncwarp();
-          const int64_t n0 = n_first + (sub + 2 * i) * 32;
-          if (row0 < p.out.rows && n0 < p.out.cols) {
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-            put_chunk<ES>(v, p.out, &maps.y, stage, bias[i], row0, n0, lane);
-          }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) remote_arrive(map_to_cta(smem_u32(&hdr->d_empty[buf]), 0));
+          else mbar_arrive(smem_u32(&hdr->d_empty[buf]));
+        }
+        __syncwarp();
         if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int64_t n0 = n_first + (sub + 2 * i) * 32;
+        if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[i], p.out, &maps.y, stage, bias[i], row0, n0, lane);
       }
     }
     __syncwarp();
@@ -246,15 +253,25 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) { cluster_arrive(); cluster_wait(); }   // neither block leaves while the other may use its memories
   if (warp == kProducers) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
-template <int BN, int ES, bool SEG>
+// scale tiles as 32-bit words: [row tile][word], a stage's 256 words of one row tile (sfa) or two (sfb)
+bool scale_map(CUtensorMap* m, const uint8_t* scales, int64_t rows, int64_t K, int box_tiles) {
+  const cuuint64_t words = static_cast<cuuint64_t>(block_tiles(K)) * (kTileBytes / 4), pitch = words * 4;
+  const cuuint64_t dims[2] = {words, static_cast<cuuint64_t>(row_tiles(rows))};
+  const cuuint32_t box[2] = {256, static_cast<cuuint32_t>(box_tiles)};
+  return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, scales, dims, &pitch, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <int BN, int ES, bool SEG, bool PAIR>
 int launch_gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& out, int64_t K, cudaStream_t st) {
-  using S = Shape<BN>;
+  using S = Shape<BN, PAIR>;
   GemmMaps maps;
   GemmParams p = {};
   p.sfa = xs;
@@ -263,32 +280,38 @@ int launch_gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const u
   p.k_tiles = static_cast<int>(block_tiles(K));
   p.row_tiles_b = static_cast<int>(row_tiles(out.cols));
   p.n_tiles = static_cast<int>((out.cols + BN - 1) / BN);
-  const int64_t tiles = row_tiles(out.rows) * p.n_tiles;
+  const int64_t tiles = (PAIR ? (row_tiles(out.rows) + 1) / 2 : row_tiles(out.rows)) * p.n_tiles;
   if (tiles > 0x7FFFFFFF - kNumSMs) return DIMQ_ERR_TOO_LARGE;
   p.tiles = static_cast<int>(tiles);
-  if (!code_map(&maps.a, xc, out.rows, K, 128) || !code_map(&maps.b, wc, out.cols, K, BN) || (out.tma && !encode_out(&maps.y, out)))
+  if (!code_map(&maps.a, xc, out.rows, K, 128) || !code_map(&maps.b, wc, out.cols, K, PAIR ? BN / 2 : BN) ||
+      (out.tma && !encode_out(&maps.y, out)) ||
+      (PAIR && (!scale_map(&maps.sfa, xs, out.rows, K, 1) || !scale_map(&maps.sfb, ws, out.cols, K, BN / 128))))
     return DIMQ_ERR_DRIVER;
   const size_t fixed = 1024 + kHeaderBytes + kEpiWarps * (ES == 2 && out.tma ? 2048 : 4096);
   p.stages = static_cast<int>((kSmemMax - fixed) / S::kStageBytes);
   if (p.stages > S::kMost) p.stages = S::kMost;
-  auto kern = mx_gemm_kernel<BN, ES, SEG>;
+  auto kern = mx_gemm_kernel<BN, ES, SEG, PAIR>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
   if (e != cudaSuccess) return static_cast<int>(e);
-  const unsigned grid = static_cast<unsigned>(tiles < kNumSMs ? tiles : kNumSMs);
-  e = launch_dependent(kern, grid, kThreads, fixed + p.stages * S::kStageBytes, st, 1, maps, p);
+  const int64_t most = PAIR ? kNumSMs / 2 : kNumSMs;
+  const unsigned grid = static_cast<unsigned>((tiles < most ? tiles : most) * (PAIR ? 2 : 1));
+  e = launch_dependent(kern, grid, kThreads, fixed + p.stages * S::kStageBytes, st, PAIR ? 2 : 1, maps, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
-// Columns a tile takes: the width that needs the fewest waves of tiles, weighed by what a 256-k step of that width costs.
+// Columns a tile takes (512: a pair of blocks): the form that needs the fewest waves of tiles, weighed by what a 256-k
+// step of it costs.
 int choose_bn(int64_t M, int64_t N) {
-  const int width[3] = {256, 128, 64};
-  const double cost[3] = {768.0, 520.0, 430.0};
+  const int form[4] = {512, 256, 128, 64};
+  const double cost[4] = {600.0, 768.0, 520.0, 430.0};
   int best = 64;
   double least = 0.0;
-  for (int i = 0; i < 3; ++i) {
-    const int64_t tiles = row_tiles(M) * ((N + width[i] - 1) / width[i]);
-    const double c = static_cast<double>((tiles + kNumSMs - 1) / kNumSMs) * cost[i];
-    if (i == 0 || c < least) { least = c; best = width[i]; }
+  for (int i = 0; i < 4; ++i) {
+    const int64_t width = form[i] > 256 ? 256 : form[i];
+    const int64_t rows = form[i] > 256 ? (row_tiles(M) + 1) / 2 : row_tiles(M), side_by_side = form[i] > 256 ? kNumSMs / 2 : kNumSMs;
+    const int64_t tiles = rows * ((N + width - 1) / width);
+    const double c = static_cast<double>((tiles + side_by_side - 1) / side_by_side) * cost[i];
+    if (i == 0 || c < least) { least = c; best = form[i]; }
   }
   return best;
 }
@@ -296,12 +319,18 @@ int choose_bn(int64_t M, int64_t N) {
 int gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& out, int64_t K, cudaStream_t st) {
   const bool wide = out.dtype == DIMQ_F32, seg = wide && block_tiles(K) > 2 * kSegStages;
   const int bn = choose_bn(out.rows, out.cols);
-#define DIMQ_MX_GEMM(BN, ES, SEG) return launch_gemm<BN, ES, SEG>(xc, xs, wc, ws, out, K, st)
-  if (seg) { if (bn == 64) DIMQ_MX_GEMM(64, 4, true); DIMQ_MX_GEMM(128, 4, true); }
-  if (wide) { if (bn == 256) DIMQ_MX_GEMM(256, 4, false); if (bn == 128) DIMQ_MX_GEMM(128, 4, false); DIMQ_MX_GEMM(64, 4, false); }
-  if (bn == 256) DIMQ_MX_GEMM(256, 2, false);
-  if (bn == 128) DIMQ_MX_GEMM(128, 2, false);
-  DIMQ_MX_GEMM(64, 2, false);
+#define DIMQ_MX_GEMM(BN, ES, SEG, PAIR) return launch_gemm<BN, ES, SEG, PAIR>(xc, xs, wc, ws, out, K, st)
+  if (seg) { if (bn == 64) DIMQ_MX_GEMM(64, 4, true, false); DIMQ_MX_GEMM(128, 4, true, false); }
+  if (wide) {
+    if (bn == 512) DIMQ_MX_GEMM(256, 4, false, true);
+    if (bn == 256) DIMQ_MX_GEMM(256, 4, false, false);
+    if (bn == 128) DIMQ_MX_GEMM(128, 4, false, false);
+    DIMQ_MX_GEMM(64, 4, false, false);
+  }
+  if (bn == 512) DIMQ_MX_GEMM(256, 2, false, true);
+  if (bn == 256) DIMQ_MX_GEMM(256, 2, false, false);
+  if (bn == 128) DIMQ_MX_GEMM(128, 2, false, false);
+  DIMQ_MX_GEMM(64, 2, false, false);
 #undef DIMQ_MX_GEMM
 }
 
