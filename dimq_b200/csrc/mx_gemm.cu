@@ -31,6 +31,7 @@ constexpr int kThreads = (kProducers + 1 + kEpiWarps) * 32;
 constexpr int kMaxStages = 8;
 constexpr int kSfCol = 256;                      // first tensor-memory column of the scales
 constexpr uint32_t kABytes = 128 * 128;
+constexpr int kBiasBytes = kEpiWarps * 4 * 128;  // four pieces of 32 columns a warp
 constexpr int kSegStages = 8;                    // fp32 results: sums of 2048 k are added up in registers
 
 struct GemmMaps {
@@ -70,7 +71,8 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t n_st = static_cast<uint32_t>(p.stages);
   GemmHeader* hdr = reinterpret_cast<GemmHeader*>(smem + n_st * S::kStageBytes);
-  unsigned char* staging = reinterpret_cast<unsigned char*>(hdr) + kHeaderBytes;
+  float* biases = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(hdr) + kHeaderBytes);
+  unsigned char* staging = reinterpret_cast<unsigned char*>(biases) + kBiasBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k_stages = (p.k_tiles + 1) / 2;
   const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
@@ -79,7 +81,7 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), PAIR ? 2 * kEpiWarps : kEpiWarps); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), PAIR ? 2 : 1); }
     hdr->abort_flag = 0u;
     fence_barrier_init();
     prefetch_tensormap(&maps.a);
@@ -197,18 +199,22 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
   } else {
     const int ew = warp - kProducers - 1;
     const int quarter = warp & 3, sub = ew >> 2;   // pieces sub, sub + 2, ... of the tile's columns
-    unsigned char* stage = staging + ew * (ES == 2 && p.out.tma ? 2048 : 4096);
-    constexpr int kChunks = BN / 32, kMine = kChunks / 2;
-    uint32_t buf = 0, bph = 0;
+    unsigned char* stage = staging + ew * kStagingBytes;
+    float* my_bias = biases + ew * 128;
+    constexpr int kMine = BN / 64;
+    uint32_t buf = 0, bph = 0, piece = 0;
     bool ok = true;
     for (int t = tile0; t < p.tiles && ok; t += tile_step) {
       const int64_t n_first = static_cast<int64_t>(t % p.n_tiles) * BN;
       const int64_t row0 = (static_cast<int64_t>(PAIR ? 2 : 1) * (t / p.n_tiles) + rank) * 128 + quarter * 32;
-      float bias[kMine];
+      if (p.out.bias != nullptr) {
+        __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int64_t n = n_first + (sub + 2 * i) * 32 + lane;
-        bias[i] = p.out.bias != nullptr && n < p.out.cols ? load_as_float(p.out.bias, p.out.bias_dtype, n) : 0.0f;
+        for (int i = 0; i < kMine; ++i) {
+          const int64_t n = n_first + (sub + 2 * i) * 32 + lane;
+          my_bias[32 * i + lane] = n < p.out.cols ? load_as_float(p.out.bias, p.out.bias_dtype, n) : 0.0f;
+        }
+        __syncwarp();
       }
       const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
       float sum[kMine][32];
@@ -231,8 +237,8 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
           tmem_ld_wait();
         }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
+        bar_sync(1, kEpiWarps * 32);      // one arrival for all: sixteen, half of them from the other block, held 18944 x 256 -> 2048 at 30 us (24)
+        if (ew == 0 && lane == 0) {
           if constexpr (PAIR) remote_arrive(map_to_cta(smem_u32(&hdr->d_empty[buf]), 0));
           else mbar_arrive(smem_u32(&hdr->d_empty[buf]));
         }
@@ -243,7 +249,8 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const int64_t n0 = n_first + (sub + 2 * i) * 32;
-        if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[i], p.out, &maps.y, stage, bias[i], row0, n0, lane);
+        const float* bias = p.out.bias != nullptr ? my_bias + 32 * i : nullptr;
+        if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[i], p.out, &maps.y, stage, piece, bias, row0, n0, lane);
       }
     }
     __syncwarp();
@@ -287,7 +294,7 @@ int launch_gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const u
       (out.tma && !encode_out(&maps.y, out)) ||
       (PAIR && (!scale_map(&maps.sfa, xs, out.rows, K, 1) || !scale_map(&maps.sfb, ws, out.cols, K, BN / 128))))
     return DIMQ_ERR_DRIVER;
-  const size_t fixed = 1024 + kHeaderBytes + kEpiWarps * (ES == 2 && out.tma ? 2048 : 4096);
+  const size_t fixed = 1024 + kHeaderBytes + kBiasBytes + kEpiWarps * kStagingBytes;
   p.stages = static_cast<int>((kSmemMax - fixed) / S::kStageBytes);
   if (p.stages > S::kMost) p.stages = S::kMost;
   auto kern = mx_gemm_kernel<BN, ES, SEG, PAIR>;

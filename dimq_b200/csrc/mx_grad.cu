@@ -40,6 +40,7 @@ struct GradParams {
   int depth_blocks;        // 64-blocks of the reduction, per term
   int terms;
   int stages, n_tiles, m_tiles;
+  int slices;              // parts of the reduction; more than one: fp32 partial results, [slice][rows][cols] at out.y
   int a_cols;              // dy's rows are the reduction (dw): its boxes are 64 columns x 64 rows
 };
 
@@ -72,6 +73,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr) : "memory");
 }
 
+struct Unit {              // a block's piece of work: a part of the reduction of one tile
+  int tile, slice, first, end;
+};
+__device__ __forceinline__ Unit unit_of(int u, int steps, const GradParams& p) {
+  Unit w;
+  w.tile = u / p.slices;
+  w.slice = u - w.tile * p.slices;
+  w.first = static_cast<int>(static_cast<int64_t>(steps) * w.slice / p.slices);
+  w.end = static_cast<int>(static_cast<int64_t>(steps) * (w.slice + 1) / p.slices);
+  return w;
+}
+
 template <int BN, int ES, bool SEG>
 __global__ void __launch_bounds__(kThreads, 1)
 mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
@@ -82,11 +95,11 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
   GradHeader* hdr = reinterpret_cast<GradHeader*>(smem + n_st * kStageBytes);
   unsigned char* staging = reinterpret_cast<unsigned char*>(hdr) + kHeaderBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int steps = p.depth_blocks * p.terms, tiles = p.n_tiles * p.m_tiles;
+  const int all_steps = p.depth_blocks * p.terms, units = p.n_tiles * p.m_tiles * p.slices;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), kEpiWarps); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), 1); }
     hdr->abort_flag = 0u;
     fence_barrier_init();
     prefetch_tensormap(&maps.a);
@@ -109,29 +122,30 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     const uint32_t turns = n_st < kProducers ? n_st : kProducers;
     uint32_t stage = 0, phase = 0, turn = 0, issued = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int n_blk = t % p.n_tiles, m_blk = t / p.n_tiles;
-      for (int term = p.terms - 1; term >= 0 && ok; --term) {
-        for (int kb = 0; kb < p.depth_blocks; ++kb) {
-          if (turn == static_cast<uint32_t>(warp)) {
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase ^ 1u, abort_flag, 0x3100u | stage))) { ok = false; break; }
-            const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * kStageBytes);
-            if (elect_one()) {
-              mbar_arrive_expect_tx(full, kStageBytes);
-              if (p.a_cols) {
-                tma_load_3d(dst, &maps.a, full, m_blk * 128, kb * kDepth, term);
-                tma_load_3d(dst + kABytes / 2, &maps.a, full, m_blk * 128 + 64, kb * kDepth, term);
-              } else {
-                tma_load_3d(dst, &maps.a, full, kb * kDepth, m_blk * 128, term);
-              }
-              tma_load_3d(dst + kABytes, &maps.b, full, 0, kb * kDepth, n_blk * (BN / 64));
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const Unit w = unit_of(u, all_steps, p);
+      const int n_blk = w.tile % p.n_tiles, m_blk = w.tile / p.n_tiles;
+      int term = p.terms - 1 - w.first / p.depth_blocks, kb = w.first % p.depth_blocks;   // smallest terms first
+      for (int s = w.first; s < w.end; ++s) {
+        if (turn == static_cast<uint32_t>(warp)) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase ^ 1u, abort_flag, 0x3100u | stage))) { ok = false; break; }
+          const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * kStageBytes);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(full, kStageBytes);
+            if (p.a_cols) {
+              tma_load_3d(dst, &maps.a, full, m_blk * 128, kb * kDepth, term);
+              tma_load_3d(dst + kABytes / 2, &maps.a, full, m_blk * 128 + 64, kb * kDepth, term);
+            } else {
+              tma_load_3d(dst, &maps.a, full, kb * kDepth, m_blk * 128, term);
             }
-            __syncwarp();
+            tma_load_3d(dst + kABytes, &maps.b, full, 0, kb * kDepth, n_blk * (BN / 64));
           }
-          ++issued;
-          if (++turn == turns) turn = 0;
-          if (++stage == n_st) { stage = 0; phase ^= 1u; }
+          __syncwarp();
         }
+        ++issued;
+        if (++turn == turns) turn = 0;
+        if (++stage == n_st) { stage = 0; phase ^= 1u; }
+        if (++kb == p.depth_blocks) { kb = 0; --term; }
       }
     }
     if (!ok && lane == 0) {   // gave up: bounded wait for the copies in flight
@@ -149,9 +163,10 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     bool ok = true;
     const uint32_t idesc = make_idesc_f16(1, 1, 128, BN) | (p.a_cols ? 1u << 15 : 0u) | (1u << 16);
     const uint64_t a_step = p.a_cols ? 2048 >> 4 : 32 >> 4;   // 16 of the reduction
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      for (int seg0 = 0; seg0 < steps && ok; seg0 += SEG ? kSegStages : steps) {
-        const int seg1 = SEG && seg0 + kSegStages < steps ? seg0 + kSegStages : steps;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const Unit w = unit_of(u, all_steps, p);
+      for (int seg0 = w.first; seg0 < w.end && ok; seg0 += SEG ? kSegStages : all_steps) {
+        const int seg1 = SEG && seg0 + kSegStages < w.end ? seg0 + kSegStages : w.end;
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_empty[buf]), bph ^ 1u, abort_flag, 0x3200u | buf))) { ok = false; break; }
         tc_fence_after();
         const uint32_t d = tmem + buf * 256;
@@ -178,15 +193,22 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
   } else {
     const int ew = warp - kProducers - 1;
     const int quarter = warp & 3, sub = ew >> 2;
-    unsigned char* stage = staging + ew * (ES == 2 && p.out.tma ? 2048 : 4096);
+    unsigned char* stage = staging + ew * kStagingBytes;
     constexpr int kMine = BN / 64;
-    uint32_t buf = 0, bph = 0;
+    uint32_t buf = 0, bph = 0, piece = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int64_t n_first = static_cast<int64_t>(t % p.n_tiles) * BN, row0 = static_cast<int64_t>(t / p.n_tiles) * 128 + quarter * 32;
+    Out out = p.out;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const Unit w = unit_of(u, all_steps, p);
+      const int64_t n_first = static_cast<int64_t>(w.tile % p.n_tiles) * BN, tile_row0 = static_cast<int64_t>(w.tile / p.n_tiles) * 128 + quarter * 32;
+      // partial results lie one under the other: a slice's rows start at slice * rows.  Only whole pieces of 32 rows go
+      // through the map; a piece that ends in the next slice's rows is stored plainly.
+      const int64_t row_off = static_cast<int64_t>(w.slice) * p.out.rows, row0 = tile_row0 + row_off;
+      out.rows = p.out.rows + row_off;
+      out.tma = p.out.tma && (p.slices == 1 || tile_row0 + 32 <= p.out.rows);
       const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
       float sum[SEG ? kMine : 1][32];
-      for (int seg0 = 0; seg0 < steps; seg0 += SEG ? kSegStages : steps) {
+      for (int seg0 = w.first; seg0 < w.end; seg0 += SEG ? kSegStages : all_steps) {
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x3500u | buf))) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
@@ -199,7 +221,7 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
               tmem_ld16(col + 16 * h, r);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) sum[i][16 * h + j] = (seg0 == 0 ? 0.0f : sum[i][16 * h + j]) + __uint_as_float(r[j]);
+              for (int j = 0; j < 16; ++j) sum[i][16 * h + j] = (seg0 == w.first ? 0.0f : sum[i][16 * h + j]) + __uint_as_float(r[j]);
             }
           } else {
             uint32_t r[32];
@@ -210,13 +232,13 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
           }
           if (i == kMine - 1) {
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&hdr->d_empty[buf]));
+            bar_sync(1, kEpiWarps * 32);
+            if (ew == 0 && lane == 0) mbar_arrive(smem_u32(&hdr->d_empty[buf]));
           }
           __syncwarp();
           if constexpr (!SEG) {
             const int64_t n0 = n_first + (sub + 2 * i) * 32;
-            if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[0], p.out, &maps.y, stage, 0.0f, row0, n0, lane);
+            if (row0 < out.rows && n0 < out.cols) put_chunk<ES>(sum[0], out, &maps.y, stage, piece, nullptr, row0, n0, lane);
           }
         }
         if (++buf == 2) { buf = 0; bph ^= 1u; }
@@ -226,7 +248,7 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
           const int64_t n0 = n_first + (sub + 2 * i) * 32;
-          if (row0 < p.out.rows && n0 < p.out.cols) put_chunk<ES>(sum[i], p.out, &maps.y, stage, 0.0f, row0, n0, lane);
+          if (row0 < out.rows && n0 < out.cols) put_chunk<ES>(sum[i], out, &maps.y, stage, piece, nullptr, row0, n0, lane);
         }
       }
     }
@@ -270,41 +292,89 @@ mx_terms_kernel(const T* __restrict__ dy, int64_t rows, int64_t cols, int64_t pi
   }
 }
 
-// Column sums: a block takes 64 columns of a run of rows, its eight warps the rows in turn; the runs' sums are added by
-// a second kernel, in order.
-constexpr int kSumRows = 512;
+// sums of the slices, in order
+template <typename T>
 __global__ void __launch_bounds__(256)
-mx_column_sum_kernel(const void* __restrict__ dy, int dtype, int64_t rows, int64_t cols, float* __restrict__ partial, void* __restrict__ out,
-                     int out_dtype) {
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 31) * 2;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
-  __shared__ float2 part[8][32];
-  float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll 8
-  for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
-    if (j < cols) s.x += load_as_float(dy, dtype, r * cols + j);
-    if (j + 1 < cols) s.y += load_as_float(dy, dtype, r * cols + j + 1);
-  }
-  part[threadIdx.x >> 5][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  for (int i = 1; i < 8; ++i) { s.x += part[i][threadIdx.x].x; s.y += part[i][threadIdx.x].y; }
-  if (gridDim.y > 1) {
-    float* p = partial + blockIdx.y * cols;
-    if (j < cols) p[j] = s.x;
-    if (j + 1 < cols) p[j + 1] = s.y;
+mx_add_slices_kernel(const float* __restrict__ partial, int slices, int64_t n, T* __restrict__ out) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  if (n % 4 == 0) {
+    float4 s = *reinterpret_cast<const float4*>(partial + i);
+    for (int r = 1; r < slices; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(partial + r * n + i);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    out[i] = from_float<T>(s.x); out[i + 1] = from_float<T>(s.y); out[i + 2] = from_float<T>(s.z); out[i + 3] = from_float<T>(s.w);
   } else {
-    if (j < cols) store_from_float(out, out_dtype, j, s.x);
-    if (j + 1 < cols) store_from_float(out, out_dtype, j + 1, s.y);
+    for (int64_t j = i; j < i + 4 && j < n; ++j) {
+      float s = partial[j];
+      for (int r = 1; r < slices; ++r) s += partial[r * n + j];
+      out[j] = from_float<T>(s);
+    }
   }
 }
+
+// Column sums: a block takes 256 columns of a run of rows, its eight warps the rows in turn; the runs' sums are added by a
+// second kernel, in order.  VEC: rows of whole 16-byte pieces, a lane has eight neighbours; else columns 32 apart.
+constexpr int kSumRows = 256;
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
+mx_column_sum_kernel(const T* __restrict__ dy, int64_t rows, int64_t cols, float* __restrict__ partial, void* __restrict__ out,
+                     int out_dtype) {
+  __shared__ float part[8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 256;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
+  float s[8] = {};
+#pragma unroll 4
+  for (int64_t r = r0 + warp; r < r1; r += 8) {
+    if (VEC) {
+      const Eight<T> e = load_pieces<T>(dy + r * cols, c0 + 8 * lane, cols);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = pair_of(e, i);
+        s[2 * i] += v.x;
+        s[2 * i + 1] += v.y;
+      }
+    } else {
+      T v[8];
+      load_neighbours<T>(dy + r * cols, c0, cols, lane, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += to_float<T>(v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[warp][VEC ? 8 * lane + i : 32 * i + lane] = s[i];
+  __syncthreads();
+  const int64_t j = c0 + threadIdx.x;
+  if (j >= cols) return;
+  float t = part[0][threadIdx.x];
+  for (int i = 1; i < 8; ++i) t += part[i][threadIdx.x];
+  if (gridDim.y > 1) partial[blockIdx.y * cols + j] = t;
+  else store_from_float(out, out_dtype, j, t);
+}
+__global__ void __launch_bounds__(128)
 mx_column_sum_finish_kernel(const float* __restrict__ partial, int64_t runs, int64_t cols, void* __restrict__ out, int out_dtype) {
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
   if (j >= cols) return;
   float s = 0.0f;
+#pragma unroll 8
   for (int64_t r = 0; r < runs; ++r) s += partial[r * cols + j];
   store_from_float(out, out_dtype, j, s);
+}
+
+template <typename T>
+int column_sum(const void* dy, int64_t M, int64_t N, float* partial, void* db, int db_dtype, cudaStream_t st) {
+  const int64_t runs = (M + kSumRows - 1) / kSumRows, gx = (N + 255) / 256;
+  if (runs > 65535) return DIMQ_ERR_TOO_LARGE;
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(runs));
+  const T* in = static_cast<const T*>(dy);
+  if ((N * static_cast<int64_t>(sizeof(T))) % 16 == 0) mx_column_sum_kernel<T, true><<<grid, 256, 0, st>>>(in, M, N, partial, db, db_dtype);
+  else mx_column_sum_kernel<T, false><<<grid, 256, 0, st>>>(in, M, N, partial, db, db_dtype);
+  const int rc = launch_status();
+  if (rc != DIMQ_OK || runs == 1) return rc;
+  mx_column_sum_finish_kernel<<<static_cast<unsigned>((N + 127) / 128), 128, 0, st>>>(partial, runs, N, db, db_dtype);
+  return launch_status();
 }
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -334,39 +404,69 @@ int split_terms(const void* dy, int dtype, int64_t M, int64_t N, void* scratch, 
 template <int BN, int ES, bool SEG>
 int launch_grad(GradMaps& maps, GradParams& p, cudaStream_t st) {
   constexpr size_t kStageBytes = kABytes + BN * kDepth * 2;
-  const size_t fixed = 1024 + kHeaderBytes + kEpiWarps * (ES == 2 && p.out.tma ? 2048 : 4096);
+  const size_t fixed = 1024 + kHeaderBytes + kEpiWarps * kStagingBytes;
   p.stages = static_cast<int>((kSmemMax - fixed) / kStageBytes);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   auto kern = mx_grad_kernel<BN, ES, SEG>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
   if (e != cudaSuccess) return static_cast<int>(e);
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.slices;
   const unsigned grid = static_cast<unsigned>(tiles < kNumSMs ? tiles : kNumSMs);
   e = launch_dependent(kern, grid, kThreads, fixed + p.stages * kStageBytes, st, 1, maps, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
-// out [R][K] = A * decoded, A = dy (reduction over its columns) or dy^T (over its rows, a_cols); `depth` values reduced
-int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms, bool a_cols, const void* decoded, int64_t depth, int64_t K,
-                 const Out& out, cudaStream_t st) {
-  GradMaps maps;
-  GradParams p = {};
-  p.out = out;
-  p.terms = terms;
-  p.a_cols = a_cols;
-  p.depth_blocks = static_cast<int>((depth + kDepth - 1) / kDepth);
-  // tile width: the fewest waves, weighed by what a stage of that width costs
+// How a product [R][K] over `depth` (times terms) is cut: tile width and slices of the reduction, by what waves of units
+// cost (cycles of a 64-step of each width) and, where it is sliced, what the partial results cost to write and to add
+// (about 3 KB a cycle over the whole chip, and a launch).  25216 tokens, 2304 x 768 weights: 54 tiles of 256 columns,
+// REPLACE us whole, REPLACE us in slices.
+struct GradPlan {
+  int bn, slices;
+};
+GradPlan plan_of(int64_t R, int64_t K, int64_t depth, int terms) {
   const int width[3] = {256, 128, 64};
   const double cost[3] = {750.0, 520.0, 430.0};
-  int bn = 256;
-  double least = 0.0;
+  const int64_t steps = (depth + kDepth - 1) / kDepth * terms;
+  GradPlan best = {256, 1};
+  double least = -1.0;
   for (int i = 0; i < 3; ++i) {
-    const int64_t t = row_tiles(out.rows) * ((K + width[i] - 1) / width[i]);
-    const double c = static_cast<double>((t + kNumSMs - 1) / kNumSMs) * cost[i];
-    if (i == 0 || c < least) { least = c; bn = width[i]; }
+    const int64_t tiles = row_tiles(R) * ((K + width[i] - 1) / width[i]);
+    for (int s = 1; s <= 16 && (s == 1 || (s * kSegStages <= steps && tiles * (s - 1) < kNumSMs)); ++s) {
+      const double waves = static_cast<double>((tiles * s + kNumSMs - 1) / kNumSMs);
+      double c = waves * (static_cast<double>((steps + s - 1) / s) * cost[i] + 2000.0);
+      if (s > 1) c += 6000.0 + static_cast<double>(R) * K * 8 * s / 3000.0;
+      if (least < 0.0 || c < least) { least = c; best = {width[i], s}; }
+    }
   }
+  return best;
+}
+int64_t slices_bytes(int64_t R, int64_t K, int64_t depth, int terms) {
+  const int s = plan_of(R, K, depth, terms).slices;
+  return s > 1 ? up(R * K * 4 * s, 256) : 0;
+}
+
+// out [R][K] = A * decoded, A = dy (reduction over its columns) or dy^T (over its rows, a_cols); `depth` values reduced
+int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms, bool a_cols, const void* decoded, int64_t depth, int64_t K,
+                 Out out, void* partial, cudaStream_t st) {
+  GradMaps maps;
+  GradParams p = {};
+  const GradPlan plan = plan_of(out.rows, K, depth, terms);
+  const int bn = plan.bn;
+  const Out result = out;
+  if (plan.slices > 1) {
+    out.y = partial;
+    out.dtype = DIMQ_F32;
+  }
+  out.tma = out_by_map(out);
+  p.out = out;
+  p.terms = terms;
+  p.slices = plan.slices;
+  p.a_cols = a_cols;
+  p.depth_blocks = static_cast<int>((depth + kDepth - 1) / kDepth);
   const int64_t n_tiles = (K + bn - 1) / bn, m_tiles = row_tiles(out.rows);
-  if (n_tiles * m_tiles > 0x7FFFFFFF - kNumSMs || static_cast<int64_t>(p.depth_blocks) * terms > 0x7FFFFFFF - 64) return DIMQ_ERR_TOO_LARGE;
+  if (n_tiles * m_tiles * plan.slices > 0x7FFFFFFF - kNumSMs || static_cast<int64_t>(p.depth_blocks) * terms > 0x7FFFFFFF - 64 ||
+      out.rows * plan.slices > 0x7FFFFF00)
+    return DIMQ_ERR_TOO_LARGE;
   p.n_tiles = static_cast<int>(n_tiles);
   p.m_tiles = static_cast<int>(m_tiles);
   const CUtensorMapDataType bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -376,18 +476,30 @@ int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms,
   const cuuint64_t bdims[3] = {64, static_cast<cuuint64_t>(depth), static_cast<cuuint64_t>(up(K, 64) / 64)};
   const cuuint64_t bstr[2] = {128, static_cast<cuuint64_t>(depth) * 128};
   const cuuint32_t bbox[3] = {64, kDepth, static_cast<cuuint32_t>(bn / 64)};
+  Out rows_of_all = out;
+  rows_of_all.rows *= plan.slices;
   if (!encode_map(&maps.a, bf16, 3, dy, adims, astr, abox, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !encode_map(&maps.b, bf16, 3, decoded, bdims, bstr, bbox, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      (out.tma && !encode_out(&maps.y, out)))
+      (out.tma && !encode_out(&maps.y, rows_of_all)))
     return DIMQ_ERR_DRIVER;
-  const bool wide = out.dtype == DIMQ_F32, seg = wide && p.depth_blocks * terms > kSegStages;
-#define DIMQ_MX_GRAD(ES, SEG)                                        \
-  return bn == 256 ? launch_grad<256, ES, SEG>(maps, p, st)          \
-         : bn == 128 ? launch_grad<128, ES, SEG>(maps, p, st) : launch_grad<64, ES, SEG>(maps, p, st)
-  if (seg) DIMQ_MX_GRAD(4, true);
-  if (wide) DIMQ_MX_GRAD(4, false);
-  DIMQ_MX_GRAD(2, false);
+  const bool wide = result.dtype == DIMQ_F32, seg = wide && p.depth_blocks * terms > kSegStages * plan.slices;
+  int rc;
+#define DIMQ_MX_GRAD(ES, SEG)                                   \
+  rc = bn == 256 ? launch_grad<256, ES, SEG>(maps, p, st)       \
+       : bn == 128 ? launch_grad<128, ES, SEG>(maps, p, st) : launch_grad<64, ES, SEG>(maps, p, st)
+  if (seg) { DIMQ_MX_GRAD(4, true); }
+  else if (out.dtype == DIMQ_F32) { DIMQ_MX_GRAD(4, false); }
+  else { DIMQ_MX_GRAD(2, false); }
 #undef DIMQ_MX_GRAD
+  if (rc != DIMQ_OK || plan.slices == 1) return rc;
+  const int64_t n = out.rows * out.cols, blocks = (n + 1023) / 1024;
+  if (blocks > 0x7FFFFFFF) return DIMQ_ERR_TOO_LARGE;
+  const unsigned grid = static_cast<unsigned>(blocks);
+  const float* from = static_cast<const float*>(partial);
+  if (wide) mx_add_slices_kernel<float><<<grid, 256, 0, st>>>(from, plan.slices, n, static_cast<float*>(result.y));
+  else if (result.dtype == DIMQ_F16) mx_add_slices_kernel<__half><<<grid, 256, 0, st>>>(from, plan.slices, n, static_cast<__half*>(result.y));
+  else mx_add_slices_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(from, plan.slices, n, static_cast<__nv_bfloat16*>(result.y));
+  return launch_status();
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K) {
@@ -397,7 +509,10 @@ int check_sizes(int64_t M, int64_t N, int64_t K) {
 }
 
 int64_t grad_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-  return decoded_bytes(M > N ? M : N, K) + terms_bytes(dtype, M, N) + partial_bytes(M, N);
+  const int terms = terms_of(dtype);
+  const int64_t in = slices_bytes(M, K, N, terms), weight = slices_bytes(N, K, M, terms), sums = partial_bytes(M, N);
+  const int64_t most = in > weight ? in : weight;
+  return decoded_bytes(M > N ? M : N, K) + terms_bytes(dtype, M, N) + (most > sums ? most : sums);
 }
 
 int clear(void* p, int dtype, int64_t n, cudaStream_t st) {   // a sum over no rows
@@ -442,8 +557,8 @@ extern "C" int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w
   rc = mx_decode_panels(w_codes, w_scales, DIMQ_MX_FP4, N, K, decoded, st);
   if (rc != DIMQ_OK) return rc;
   mx::Out out = {dx, nullptr, nullptr, M, K, 0, dx_dtype, DIMQ_EPI_NONE, 0};
-  out.tma = mx::out_by_map(out);
-  return grad_product(a, M, N, pitch, terms_of(dy_dtype), false, decoded, N, K, out, st);
+  return grad_product(a, M, N, pitch, terms_of(dy_dtype), false, decoded, N, K, out,
+                      decoded + decoded_bytes(M > N ? M : N, K) + terms_bytes(dy_dtype, M, N), st);
 }
 
 extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_codes, const uint8_t* x_scales, int format, void* dw,
@@ -466,14 +581,10 @@ extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_c
   unsigned char* terms = decoded + decoded_bytes(M > N ? M : N, K);
   float* partial = reinterpret_cast<float*>(terms + terms_bytes(dy_dtype, M, N));
   if (db != nullptr) {
-    const int64_t runs = (M + kSumRows - 1) / kSumRows, gx = (N + 63) / 64;
-    if (runs > 65535) return DIMQ_ERR_TOO_LARGE;
-    mx_column_sum_kernel<<<dim3(static_cast<unsigned>(gx), static_cast<unsigned>(runs)), 256, 0, st>>>(dy, dy_dtype, M, N, partial, db, db_dtype);
-    if ((rc = launch_status()) != DIMQ_OK) return rc;
-    if (runs > 1) {
-      mx_column_sum_finish_kernel<<<static_cast<unsigned>((N + 255) / 256), 256, 0, st>>>(partial, runs, N, db, db_dtype);
-      if ((rc = launch_status()) != DIMQ_OK) return rc;
-    }
+    rc = dy_dtype == DIMQ_F32 ? column_sum<float>(dy, M, N, partial, db, db_dtype, st)
+         : dy_dtype == DIMQ_F16 ? column_sum<__half>(dy, M, N, partial, db, db_dtype, st)
+                                : column_sum<__nv_bfloat16>(dy, M, N, partial, db, db_dtype, st);
+    if (rc != DIMQ_OK) return rc;
   }
   if (dw == nullptr) return DIMQ_OK;
   const void* a;
@@ -483,6 +594,5 @@ extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_c
   rc = mx_decode_panels(x_codes, x_scales, format, M, K, decoded, st);
   if (rc != DIMQ_OK) return rc;
   mx::Out out = {dw, nullptr, nullptr, N, K, 0, dw_dtype, DIMQ_EPI_NONE, 0};
-  out.tma = mx::out_by_map(out);
-  return grad_product(a, M, N, pitch, terms_of(dy_dtype), true, decoded, M, K, out, st);
+  return grad_product(a, M, N, pitch, terms_of(dy_dtype), true, decoded, M, K, out, partial, st);
 }

@@ -183,17 +183,28 @@ __device__ __forceinline__ float element(const uint4& q, int i, int dtype) {
   return dtype == DIMQ_BF16 ? __uint_as_float(static_cast<uint32_t>(h) << 16) : __half2float(__ushort_as_half(h));
 }
 
-// Sums of 32 rows x 32 columns (lane = row, v = its columns from n0 on) -> y.  `bias` is that of column n0 + lane.
-// stage: this warp's piece of shared memory, 1024-aligned (ES = 2 through the map: 2 KB, else 4 KB).
+// Shared memory of an epilogue warp: two pieces of 2 KB that map stores read in turn (16-bit results), or one of 4 KB
+// (fp32: a second one would cost the ring a stage).
+constexpr uint32_t kStagingBytes = 4096;
+
+// Sums of 32 rows x 32 columns (lane = row, v = its columns from n0 on) -> y.  bias: 32 floats in shared memory, or null.
+// stage: this warp's shared memory, 1024-aligned; turn: which piece is next.
 // With a map: bias, activation and residual on the lane's row, packed into the swizzled box the map stores.  Without: the
-// sums change hands through shared memory, so that a warp stores 32 neighbours of one row at a time.
+// sums change hands through shared memory, so that a warp stores 32 neighbours of one row at a time.  (Boxes of 64 columns,
+// and 16-byte stores of four rows at a time instead of the map, were slower: 25216 x 768 -> 2304 bf16 59 and 69 us against
+// 57.)
 template <int ES>
-__device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CUtensorMap* map, unsigned char* stage, float bias,
-                                          int64_t row0, int64_t n0, int lane) {
+__device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CUtensorMap* map, unsigned char* stage, uint32_t& turn,
+                                          const float* bias, int64_t row0, int64_t n0, int lane) {
   if (o.tma) {
     const int64_t row = row0 + lane;
+    if (bias != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, bias, j);
+      for (int j = 0; j < 8; ++j) {
+        const float4 b = *reinterpret_cast<const float4*>(bias + 4 * j);   // one address for all lanes
+        v[4 * j] += b.x; v[4 * j + 1] += b.y; v[4 * j + 2] += b.z; v[4 * j + 3] += b.w;
+      }
+    }
     if (o.residual != nullptr) {
       constexpr int kPer = 16 / ES;
       const char* r = static_cast<const char*>(o.residual) + (row * o.cols + n0) * ES;
@@ -211,7 +222,13 @@ __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CU
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = max_nan(v[j], 0.0f);
     }
-    if (elect_one()) tma_store_wait_read();   // the last store has read this piece
+    if (ES == 2) {
+      stage += turn * 2048;
+      turn ^= 1u;
+      if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the store before the last has read this piece
+    } else if (elect_one()) {
+      tma_store_wait_read();
+    }
     __syncwarp();
     if (ES == 2) {   // 64-byte rows, 64-byte swizzle
       unsigned char* p = stage + lane * 64;
@@ -243,18 +260,20 @@ __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CU
     return;
   }
   float* f = reinterpret_cast<float*>(stage);
+  if (elect_one()) tma_store_wait_read();   // pieces stored through a map before this one
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < 32; ++j) f[lane * 32 + (j ^ lane)] = v[j];
   __syncwarp();
   const int64_t n = n0 + lane;
+  const float b = bias != nullptr ? bias[lane] : 0.0f;
   if (n < o.cols) {
     const int rows = static_cast<int>(o.rows - row0 < 32 ? o.rows - row0 : 32);
 #pragma unroll 4
     for (int r = 0; r < rows; ++r) {
       const int64_t at = (row0 + r) * o.cols + n;
       const float res = o.residual != nullptr ? load_as_float(o.residual, o.dtype, at) : 0.0f;
-      store_from_float(o.y, o.dtype, at, activate_any(f[r * 32 + (lane ^ r)] + bias, res, o.epilogue));
+      store_from_float(o.y, o.dtype, at, activate_any(f[r * 32 + (lane ^ r)] + b, res, o.epilogue));
     }
   }
   __syncwarp();

@@ -223,7 +223,7 @@ def test_linear_rows_do_not_depend_on_their_neighbours(cuda_device, m):
 
 # ---- gradients ------------------------------------------------------------------------------------
 
-GRADS = [(1, 1, 1), (1, 64, 32), (3, 33, 7), (64, 128, 64), (130, 260, 129), (100, 1000, 72), (513, 96, 200), (257, 300, 515), (2000, 64, 40), (700, 2600, 1300)]
+GRADS = [(1, 1, 1), (1, 64, 32), (3, 33, 7), (64, 128, 64), (130, 260, 129), (100, 1000, 72), (513, 96, 200), (257, 300, 515), (2000, 64, 40), (700, 2600, 1300), (9000, 200, 264), (40, 136, 5000)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
