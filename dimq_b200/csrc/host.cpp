@@ -13,6 +13,8 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -725,6 +727,11 @@ Tensor attention_qkv(const Tensor& qkv, int64_t heads, int* launches) {
   return y;
 }
 
+void count_launches_no_gil(int n) {
+  pybind11::gil_scoped_acquire gil;
+  count_launches(n);
+}
+
 // ---- microscaled numbers ----------------------------------------------------------------------------
 
 struct MxSizes {
@@ -845,14 +852,29 @@ Tensor mx_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, con
   return y;
 }
 
+// A quantised matrix in one buffer, for the library's own use: codes, then (on 512 bytes) scales.
+struct MxBuffer {
+  Tensor t;
+  int64_t scales_at = 0;
+  uint8_t* codes() const { return static_cast<uint8_t*>(t.data_ptr()); }
+  uint8_t* scales() const { return codes() + scales_at; }
+};
+int64_t mx_scales_at(int64_t rows, const MxSizes& s) { return (rows * s.pitch + 511) / 512 * 512; }
+MxBuffer mx_buffer(int64_t rows, int64_t cols, int format, const Tensor& like) {
+  const MxSizes s = mx_sizes(rows, cols, format);
+  MxBuffer b;
+  b.scales_at = mx_scales_at(rows, s);
+  b.t = scratch(b.scales_at + s.scale_bytes, like);
+  return b;
+}
+
 // The layer's forward for training: y, what its backward needs of x (keep: 0 nothing, else the format) and of w.
 struct MxForward {
   Tensor y;
-  OptTensor x_codes, x_scales;
-  Mx w;
+  Tensor x, w;     // undefined: not kept
 };
 
-MxForward mx_layer_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, int keep, int* launches) {
+MxForward mx_layer_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, int keep, bool keep_w, int* launches) {
   require_cuda(x, "mx_linear");
   require_cuda(weight, "mx_linear");
   same_device(weight, x, "weight");
@@ -865,27 +887,23 @@ MxForward mx_layer_forward(const Tensor& x, const Tensor& weight, const OptTenso
   void* st = stream_of(x);
   const Tensor xc = x.contiguous(), wc = weight.contiguous();
   const int64_t m = mx_rows(x, k);
-  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  const MxBuffer w4 = mx_buffer(n, k, DIMQ_MX_FP4, x), x4 = mx_buffer(m, k, DIMQ_MX_FP4, x);
   MxForward f;
-  f.w = mx_empty({n}, n, k, DIMQ_MX_FP4, x);
-  check(dimq_mx_quantize(wc.data_ptr(), wd, n, k, DIMQ_MX_FP4, f.w.codes.data_ptr(), writable(f.w.scales), st), "mx_quantize");
-  Mx x4 = mx_empty(lead, m, k, DIMQ_MX_FP4, x);
+  check(dimq_mx_quantize(wc.data_ptr(), wd, n, k, DIMQ_MX_FP4, w4.codes(), w4.scales(), st), "mx_quantize");
   if (keep == DIMQ_MX_INT8) {
-    Mx x8 = mx_empty(lead, m, k, DIMQ_MX_INT8, x);
-    check(dimq_mx_quantize_both(xc.data_ptr(), xd, m, k, writable(x4.codes), writable(x4.scales),
-                                static_cast<int8_t*>(x8.codes.data_ptr()), writable(x8.scales), st), "mx_quantize_both");
-    f.x_codes = x8.codes;
-    f.x_scales = x8.scales;
+    const MxBuffer x8 = mx_buffer(m, k, DIMQ_MX_INT8, x);
+    check(dimq_mx_quantize_both(xc.data_ptr(), xd, m, k, x4.codes(), x4.scales(), reinterpret_cast<int8_t*>(x8.codes()), x8.scales(), st),
+          "mx_quantize_both");
+    f.x = x8.t;
   } else {
-    check(dimq_mx_quantize(xc.data_ptr(), xd, m, k, DIMQ_MX_FP4, x4.codes.data_ptr(), writable(x4.scales), st), "mx_quantize");
-    if (keep == DIMQ_MX_FP4) {
-      f.x_codes = x4.codes;
-      f.x_scales = x4.scales;
-    }
+    check(dimq_mx_quantize(xc.data_ptr(), xd, m, k, DIMQ_MX_FP4, x4.codes(), x4.scales(), st), "mx_quantize");
+    if (keep == DIMQ_MX_FP4) f.x = x4.t;
   }
-  *launches += 1 + (m > 0);
+  if (keep_w) f.w = w4.t;
   f.y = at::empty(out_shape(x, n), x.options().memory_format(at::MemoryFormat::Contiguous));
-  mx_linear_into(x4.codes, 0, x4.scales, f.w, b, std::nullopt, f.y, m, n, k, DIMQ_EPI_NONE, launches);
+  check(dimq_mx_linear(x4.codes(), 0, x4.scales(), w4.codes(), w4.scales(), ptr(b.t), b.dtype, nullptr, f.y.data_ptr(),
+                       dtype_code(f.y, "y"), m, n, k, DIMQ_EPI_NONE, nullptr, 0, st), "mx_linear");
+  *launches += 1 + 2 * (m > 0);
   return f;
 }
 
@@ -914,10 +932,7 @@ Tensor mx_grad_input(const Tensor& dy, const Tensor& codes, const Tensor& scales
   return dx;
 }
 
-// (dw, db): dw where dw_dtype, db where db_dtype is given
-std::pair<OptTensor, OptTensor> mx_grad_weight(const Tensor& dy, const Tensor& codes, const Tensor& scales, int64_t k, int format,
-                                               std::optional<at::ScalarType> dw_dtype, std::optional<at::ScalarType> db_dtype,
-                                               int* launches) {
+Tensor mx_grad_weight(const Tensor& dy, const Tensor& codes, const Tensor& scales, int64_t k, int format, at::ScalarType dt, int* launches) {
   require_cuda(dy, "mx_linear_grad_weight");
   const int dyd = dtype_code(dy, "grad");
   if (dy.dim() == 0 || dy.size(-1) <= 0) fail("mx_linear_grad_weight expects a last dimension of out_features");
@@ -928,34 +943,85 @@ std::pair<OptTensor, OptTensor> mx_grad_weight(const Tensor& dy, const Tensor& c
   same_device(codes, dy, "activation codes");
   const Mx x = mx_operand(codes, scales, &m, k, format, "activation");
   const Tensor g = aligned16(dy);
-  OptTensor dw, db;
-  const auto opt = dy.options().memory_format(at::MemoryFormat::Contiguous);
-  if (dw_dtype.has_value()) dw = at::empty({n, k}, opt.dtype(*dw_dtype));
-  if (db_dtype.has_value()) db = at::empty({n}, opt.dtype(*db_dtype));
+  Tensor dw = at::empty({n, k}, dy.options().dtype(dt).memory_format(at::MemoryFormat::Contiguous));
   int64_t need = 0;
   const Tensor ws = mx_grad_scratch(g, dyd, m, n, k, &need);
-  check(dimq_mx_grad_weight(g.data_ptr(), dyd, x.codes.data_ptr(), bytes_of(x.scales), format, dw.has_value() ? dw->data_ptr() : nullptr,
-                            dw.has_value() ? dtype_code(*dw, "out_dtype") : 0, db.has_value() ? db->data_ptr() : nullptr,
-                            db.has_value() ? dtype_code(*db, "bias dtype") : 0, m, n, k, ws.data_ptr(), need, stream_of(dy)),
-        "mx_linear_grad_weight");
-  *launches += (dw.has_value() ? 2 : 0) + (db.has_value() ? 1 : 0);
-  return {dw, db};
+  check(dimq_mx_grad_weight(g.data_ptr(), dyd, x.codes.data_ptr(), bytes_of(x.scales), format, dw.data_ptr(), dtype_code(dw, "out_dtype"),
+                            nullptr, 0, m, n, k, ws.data_ptr(), need, stream_of(dy)), "mx_linear_grad_weight");
+  *launches += m > 0 ? 2 : 0;
+  return dw;
 }
 
-Tensor mx_column_sum(const Tensor& dy, at::ScalarType dt, int* launches) {
-  require_cuda(dy, "mx_column_sum");
-  const int dyd = dtype_code(dy, "grad");
-  if (dy.dim() == 0 || dy.size(-1) <= 0) fail("mx_column_sum expects a last dimension of out_features");
-  const c10::cuda::CUDAGuard guard(dy.device());
-  const Tensor g = aligned16(dy);
-  const int64_t n = dy.size(-1), m = mx_rows(dy, n);
-  Tensor db = at::empty({n}, dy.options().dtype(dt).memory_format(at::MemoryFormat::Contiguous));
-  int64_t need = 0;
-  const Tensor ws = mx_grad_scratch(g, dyd, m, n, 1, &need);
-  check(dimq_mx_grad_weight(g.data_ptr(), dyd, nullptr, nullptr, DIMQ_MX_INT8, nullptr, 0, db.data_ptr(), dtype_code(db, "bias dtype"),
-                            m, n, 1, ws.data_ptr(), need, stream_of(dy)), "mx_linear_grad_weight");
-  *launches += 1;
-  return db;
+// Gradients straight through the rounding, from what the forward kept.  Differentiable once: a second derivative raises.
+class MxLayer : public torch::autograd::Function<MxLayer> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias, int64_t keep,
+                        bool need_x, bool need_w) {
+    int launches = 0;
+    MxForward f = mx_layer_forward(x, weight, bias, need_w ? static_cast<int>(keep) : 0, need_x, &launches);
+    count_launches_no_gil(launches);
+    ctx->save_for_backward({f.x, f.w});
+    ctx->saved_data["keep"] = keep;
+    ctx->saved_data["n"] = weight.size(0);
+    ctx->saved_data["k"] = weight.size(1);
+    ctx->saved_data["x"] = static_cast<int64_t>(x.scalar_type());
+    ctx->saved_data["w"] = static_cast<int64_t>(weight.scalar_type());
+    ctx->saved_data["b"] = bias.has_value() ? static_cast<int64_t>(bias->scalar_type()) : int64_t{-1};
+    return f.y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
+    const int keep = static_cast<int>(ctx->saved_data["keep"].toInt());
+    const auto type = [&](const char* name) { return static_cast<at::ScalarType>(ctx->saved_data[name].toInt()); };
+    torch::autograd::variable_list out(6);
+    if (!grads[0].defined()) return out;
+    const Tensor& dy = grads[0];
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = ctx->saved_data["b"].toInt() >= 0 && ctx->needs_input_grad(2);
+    const c10::cuda::CUDAGuard guard(dy.device());
+    const int dyd = dtype_code(dy, "grad");
+    const Tensor g = aligned16(dy.detach());
+    const int64_t m = mx_rows(g, n);
+    const auto opt = g.options().memory_format(at::MemoryFormat::Contiguous);
+    Tensor dx, dw, db;
+    if (need_x) dx = at::empty(out_shape(g, k), opt.dtype(type("x")));
+    if (need_w) dw = at::empty({n, k}, opt.dtype(type("w")));
+    if (need_b) db = at::empty({n}, opt.dtype(type("b")));
+    if (!need_x && !need_w && !need_b) return out;
+    MxBuffer x, w;
+    if (need_w) x = {saved[0], mx_scales_at(m, mx_sizes(m, k, keep))};
+    if (need_x) w = {saved[1], mx_scales_at(n, mx_sizes(n, k, DIMQ_MX_FP4))};
+    int64_t need = 0;
+    check(dimq_mx_grad_workspace_bytes(dyd, m, n, k, &need), "mx_grad_workspace_bytes");
+    const Tensor ws = scratch(need, g);
+    const auto at_or_null = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const auto dtype_of = [](const Tensor& t) { return t.defined() ? dtype_code(t, "gradient") : 0; };
+    if (m > 0 || need_w || need_b)
+      check(dimq_mx_grads(g.data_ptr(), dyd, need_x ? w.codes() : nullptr, need_x ? w.scales() : nullptr, need_w ? x.codes() : nullptr,
+                          need_w ? x.scales() : nullptr, keep, at_or_null(dx), dtype_of(dx), at_or_null(dw), dtype_of(dw), at_or_null(db),
+                          dtype_of(db), m, n, k, ws.data_ptr(), need, stream_of(g)), "mx_grads");
+    count_launches_no_gil(m > 0 ? 2 * need_x + 2 * need_w + need_b : 0);
+    out[0] = dx;
+    out[1] = dw;
+    out[2] = db;
+    if (at::GradMode::is_enabled()) {     // create_graph: whoever differentiates these again is told
+      torch::autograd::variable_list parts;
+      for (auto& t : out)
+        if (t.defined()) parts.push_back(t.detach().requires_grad_(true));
+      auto error = std::make_shared<torch::autograd::DelayedError>("mx_linear is differentiable once", static_cast<int64_t>(parts.size()));
+      parts = (*error)(std::move(parts));
+      size_t i = 0;
+      for (auto& t : out)
+        if (t.defined()) t = parts[i++];
+    }
+    return out;
+  }
+};
+
+Tensor mx_layer(const Tensor& x, const Tensor& weight, const OptTensor& bias, int keep) {
+  const bool grad = at::GradMode::is_enabled();
+  return MxLayer::apply(x, weight, bias, keep, grad && x.requires_grad(), grad && weight.requires_grad());
 }
 
 // ---- the Python module ----------------------------------------------------------------------------
@@ -1210,29 +1276,15 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* tuple_of(const std::vector<OptTensor>& v) {
-  PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(v.size()));
-  if (t == nullptr) return nullptr;
-  for (size_t i = 0; i < v.size(); ++i) {
-    PyObject* o = wrap(v[i]);
-    if (o == nullptr) { Py_DECREF(t); return nullptr; }
-    PyTuple_SET_ITEM(t, static_cast<Py_ssize_t>(i), o);
-  }
-  return t;
-}
-
-PyObject* py_mx_layer_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* py_mx_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  ARGS(4, "mx_layer_forward");
+  ARGS(4, "mx_layer");
   const Tensor x = as_tensor(a[0]), weight = as_tensor(a[1]);
   const OptTensor bias = as_opt_tensor(a[2]);
-  const int64_t k = as_int(a[3]);
-  const int keep = k == 0 ? 0 : mx_format(k);
-  int launches = 0;
-  MxForward f;
-  { NO_GIL; f = mx_layer_forward(x, weight, bias, keep, &launches); }
-  count_launches(launches);
-  return tuple_of({f.y, f.x_codes, f.x_scales, f.w.codes, f.w.scales});
+  const int keep = mx_format(as_int(a[3]));
+  Tensor y;
+  { NO_GIL; y = mx_layer(x, weight, bias, keep); }
+  return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
@@ -1252,41 +1304,21 @@ PyObject* py_mx_grad_input(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyObject* py_mx_grad_weight(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  ARGS(7, "mx_grad_weight");
+  ARGS(6, "mx_grad_weight");
   const Tensor dy = as_tensor(a[0]), codes = as_tensor(a[1]), scales = as_tensor(a[2]);
   const int64_t k = as_int(a[3]);
   const int format = mx_format(as_int(a[4]));
-  std::optional<at::ScalarType> dw, db;
-  if (a[5] != Py_None) dw = as_dtype(a[5]);
-  if (a[6] != Py_None) db = as_dtype(a[6]);
+  const at::ScalarType dt = as_dtype(a[5]);
   int launches = 0;
-  std::pair<OptTensor, OptTensor> g;
-  { NO_GIL; g = mx_grad_weight(dy, codes, scales, k, format, dw, db, &launches); }
+  Tensor dw;
+  { NO_GIL; dw = mx_grad_weight(dy, codes, scales, k, format, dt, &launches); }
   count_launches(launches);
-  return pair_of(g.first, g.second);
-  END_HANDLE_TH_ERRORS
-}
-
-PyObject* py_mx_column_sum(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  ARGS(2, "mx_column_sum");
-  const Tensor dy = as_tensor(a[0]);
-  const at::ScalarType dt = as_dtype(a[1]);
-  int launches = 0;
-  Tensor db;
-  { NO_GIL; db = mx_column_sum(dy, dt, &launches); }
-  count_launches(launches);
-  return THPVariable_Wrap(db);
+  return THPVariable_Wrap(dw);
   END_HANDLE_TH_ERRORS
 }
 
 // ---- torch.ops.dimq: the kernels of the CUDA key for the schemas dimq_b200/ops.py defines ---------------
 // (the dispatcher calls these without the GIL)
-
-void count_launches_no_gil(int n) {
-  pybind11::gil_scoped_acquire gil;
-  count_launches(n);
-}
 
 Tensor op_pack_u4(const Tensor& indices) {
   int launches = 0;
@@ -1432,8 +1464,8 @@ PyObject* py_capturing(PyObject*, PyObject* device) {
 PyMethodDef kMethods[] = {FAST(linear_wq), FAST(linear_a4), FAST(conv2d_wq), FAST(conv2d_a4),
                           FAST(hard_quantize), FAST(fake_quantize_ste), FAST(unpack_bits), FAST(pack_bits), FAST(add_layer_norm),
                           FAST(max_pool_nhwc), FAST(images_to_nhwc), FAST(attention_qkv),
-                          FAST(mx_quantize), FAST(mx_dequantize), FAST(mx_linear), FAST(mx_layer_forward), FAST(mx_grad_input),
-                          FAST(mx_grad_weight), FAST(mx_column_sum),
+                          FAST(mx_quantize), FAST(mx_dequantize), FAST(mx_linear), FAST(mx_layer), FAST(mx_grad_input),
+                          FAST(mx_grad_weight),
                           {"set_launch_count", py_set_launch_count, METH_O, nullptr},
                           {"set_ops", py_set_ops, METH_O, nullptr},
                           {"record_event", py_record_event, METH_O, nullptr},

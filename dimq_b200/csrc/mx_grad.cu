@@ -538,38 +538,22 @@ extern "C" int dimq_mx_grad_workspace_bytes(int dy_dtype, int64_t M, int64_t N, 
   return DIMQ_OK;
 }
 
-extern "C" int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, void* dx,
-                                  int dx_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
-                                  void* stream) {
+// dx (null: not wanted) from w, dw (null) from x, db (null); dy's terms are made once
+static int grads(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, const void* x_codes,
+                 const uint8_t* x_scales, int format, void* dx, int dx_dtype, void* dw, int dw_dtype, void* db, int db_dtype, int64_t M,
+                 int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = check_sizes(M, N, K);
   if (rc != DIMQ_OK) return rc;
-  if (!valid_dtype(dy_dtype) || !valid_dtype(dx_dtype)) return DIMQ_ERR_BAD_DTYPE;
-  if (M == 0) return DIMQ_OK;
-  if (dy == nullptr || w_codes == nullptr || w_scales == nullptr || dx == nullptr) return DIMQ_ERR_NULL_POINTER;
-  if (!aligned(dy, 16) || !aligned(w_codes, 16) || !aligned(w_scales, 16) || !aligned(workspace, 256)) return DIMQ_ERR_ALIGNMENT;
-  if (workspace == nullptr || workspace_bytes < grad_bytes(dy_dtype, M, N, K)) return DIMQ_ERR_SCRATCH_TOO_SMALL;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  unsigned char* decoded = static_cast<unsigned char*>(workspace);
-  const void* a;
-  int64_t pitch;
-  rc = split_terms(dy, dy_dtype, M, N, decoded + decoded_bytes(M > N ? M : N, K), &a, &pitch, st);
-  if (rc != DIMQ_OK) return rc;
-  rc = mx_decode_panels(w_codes, w_scales, DIMQ_MX_FP4, N, K, decoded, st);
-  if (rc != DIMQ_OK) return rc;
-  mx::Out out = {dx, nullptr, nullptr, M, K, 0, dx_dtype, DIMQ_EPI_NONE, 0};
-  return grad_product(a, M, N, pitch, terms_of(dy_dtype), false, decoded, N, K, out,
-                      decoded + decoded_bytes(M > N ? M : N, K) + terms_bytes(dy_dtype, M, N), st);
-}
-
-extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_codes, const uint8_t* x_scales, int format, void* dw,
-                                   int dw_dtype, void* db, int db_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
-                                   int64_t workspace_bytes, void* stream) {
-  int rc = check_sizes(M, N, K);
-  if (rc != DIMQ_OK) return rc;
-  if (!mx::valid_format(format)) return DIMQ_ERR_BAD_BITS;
-  if (!valid_dtype(dy_dtype) || (dw != nullptr && !valid_dtype(dw_dtype)) || (db != nullptr && !valid_dtype(db_dtype))) return DIMQ_ERR_BAD_DTYPE;
-  if ((dw == nullptr && db == nullptr) || (M > 0 && (dy == nullptr || (dw != nullptr && (x_codes == nullptr || x_scales == nullptr))))) return DIMQ_ERR_NULL_POINTER;
-  if (!aligned(dy, 16) || !aligned(x_codes, 16) || !aligned(x_scales, 16) || !aligned(workspace, 256)) return DIMQ_ERR_ALIGNMENT;
+  if (dw != nullptr && !mx::valid_format(format)) return DIMQ_ERR_BAD_BITS;
+  if (!valid_dtype(dy_dtype) || (dx != nullptr && !valid_dtype(dx_dtype)) || (dw != nullptr && !valid_dtype(dw_dtype)) ||
+      (db != nullptr && !valid_dtype(db_dtype)))
+    return DIMQ_ERR_BAD_DTYPE;
+  if (M > 0 && (dy == nullptr || (dx != nullptr && (w_codes == nullptr || w_scales == nullptr)) ||
+                (dw != nullptr && (x_codes == nullptr || x_scales == nullptr))))
+    return DIMQ_ERR_NULL_POINTER;
+  if (!aligned(dy, 16) || !aligned(w_codes, 16) || !aligned(w_scales, 16) || !aligned(x_codes, 16) || !aligned(x_scales, 16) ||
+      !aligned(workspace, 256))
+    return DIMQ_ERR_ALIGNMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (M == 0) {
     if (dw != nullptr) rc = clear(dw, dw_dtype, N * K, st);
@@ -578,21 +562,54 @@ extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_c
   }
   if (workspace == nullptr || workspace_bytes < grad_bytes(dy_dtype, M, N, K)) return DIMQ_ERR_SCRATCH_TOO_SMALL;
   unsigned char* decoded = static_cast<unsigned char*>(workspace);
-  unsigned char* terms = decoded + decoded_bytes(M > N ? M : N, K);
-  float* partial = reinterpret_cast<float*>(terms + terms_bytes(dy_dtype, M, N));
+  unsigned char* split = decoded + decoded_bytes(M > N ? M : N, K);
+  float* partial = reinterpret_cast<float*>(split + terms_bytes(dy_dtype, M, N));
   if (db != nullptr) {
     rc = dy_dtype == DIMQ_F32 ? column_sum<float>(dy, M, N, partial, db, db_dtype, st)
          : dy_dtype == DIMQ_F16 ? column_sum<__half>(dy, M, N, partial, db, db_dtype, st)
                                 : column_sum<__nv_bfloat16>(dy, M, N, partial, db, db_dtype, st);
     if (rc != DIMQ_OK) return rc;
   }
-  if (dw == nullptr) return DIMQ_OK;
+  if (dx == nullptr && dw == nullptr) return DIMQ_OK;
   const void* a;
   int64_t pitch;
-  rc = split_terms(dy, dy_dtype, M, N, terms, &a, &pitch, st);
+  const int terms = terms_of(dy_dtype);
+  rc = split_terms(dy, dy_dtype, M, N, split, &a, &pitch, st);
   if (rc != DIMQ_OK) return rc;
-  rc = mx_decode_panels(x_codes, x_scales, format, M, K, decoded, st);
-  if (rc != DIMQ_OK) return rc;
-  mx::Out out = {dw, nullptr, nullptr, N, K, 0, dw_dtype, DIMQ_EPI_NONE, 0};
-  return grad_product(a, M, N, pitch, terms_of(dy_dtype), true, decoded, M, K, out, partial, st);
+  if (dx != nullptr) {
+    rc = mx_decode_panels(w_codes, w_scales, DIMQ_MX_FP4, N, K, decoded, st);
+    if (rc != DIMQ_OK) return rc;
+    rc = grad_product(a, M, N, pitch, terms, false, decoded, N, K, {dx, nullptr, nullptr, M, K, 0, dx_dtype, DIMQ_EPI_NONE, 0}, partial, st);
+    if (rc != DIMQ_OK) return rc;
+  }
+  if (dw != nullptr) {
+    rc = mx_decode_panels(x_codes, x_scales, format, M, K, decoded, st);
+    if (rc != DIMQ_OK) return rc;
+    rc = grad_product(a, M, N, pitch, terms, true, decoded, M, K, {dw, nullptr, nullptr, N, K, 0, dw_dtype, DIMQ_EPI_NONE, 0}, partial, st);
+  }
+  return rc;
+}
+
+extern "C" int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, void* dx,
+                                  int dx_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
+  if (dx == nullptr && M > 0) return DIMQ_ERR_NULL_POINTER;
+  return grads(dy, dy_dtype, w_codes, w_scales, nullptr, nullptr, 0, dx, dx_dtype, nullptr, 0, nullptr, 0, M, N, K, workspace,
+               workspace_bytes, stream);
+}
+
+extern "C" int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_codes, const uint8_t* x_scales, int format, void* dw,
+                                   int dw_dtype, void* db, int db_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+  if (dw == nullptr && db == nullptr) return DIMQ_ERR_NULL_POINTER;
+  return grads(dy, dy_dtype, nullptr, nullptr, x_codes, x_scales, format, nullptr, 0, dw, dw_dtype, db, db_dtype, M, N, K, workspace,
+               workspace_bytes, stream);
+}
+
+extern "C" int dimq_mx_grads(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, const void* x_codes,
+                             const uint8_t* x_scales, int format, void* dx, int dx_dtype, void* dw, int dw_dtype, void* db, int db_dtype,
+                             int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (dx == nullptr && dw == nullptr && db == nullptr) return DIMQ_ERR_NULL_POINTER;
+  return grads(dy, dy_dtype, w_codes, w_scales, x_codes, x_scales, format, dx, dx_dtype, dw, dw_dtype, db, db_dtype, M, N, K, workspace,
+               workspace_bytes, stream);
 }

@@ -666,7 +666,7 @@ def mx_linear_grad_weight(grad: torch.Tensor, codes: torch.Tensor, scales: torch
                           fmt: str = "int8", *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``grad.T @ x`` (over all leading dimensions) for the activations that ``mx_quantize(x, fmt)`` keeps in
     ``codes`` / ``scales``: the gradient of a linear layer's weight, ``[out_features, in_features]``."""
-    return _lib.host().mx_grad_weight(grad, codes, scales, in_features, _mx_format(fmt), out_dtype or torch.float32, None)[0]
+    return _lib.host().mx_grad_weight(grad, codes, scales, in_features, _mx_format(fmt), out_dtype)
 
 
 def last_device_status() -> int:

@@ -48,34 +48,6 @@ def fake_quant_activation(x: torch.Tensor, activation_centers: torch.Tensor, chu
     return _FakeQuantSTE.apply(x, activation_centers, None)
 
 
-class _MXLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, keep: int):
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        y, x_codes, x_scales, w_codes, w_scales = _lib.host().mx_layer_forward(x, weight, bias, keep if need_w else 0)
-        if not need_x:
-            w_codes = w_scales = None
-        ctx.save_for_backward(x_codes, x_scales, w_codes, w_scales)
-        ctx.keep, ctx.in_features = keep, weight.shape[1]
-        ctx.dtypes = x.dtype, weight.dtype, bias.dtype if need_b else None
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad: torch.Tensor):
-        x_codes, x_scales, w_codes, w_scales = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        x_dtype, w_dtype, b_dtype = ctx.dtypes
-        host = _lib.host()
-        dx = host.mx_grad_input(grad, w_codes, w_scales, ctx.in_features, x_dtype) if need_x else None
-        dw = db = None
-        if need_w:
-            dw, db = host.mx_grad_weight(grad, x_codes, x_scales, ctx.in_features, ctx.keep, w_dtype, b_dtype)
-        elif need_b:
-            db = host.mx_column_sum(grad, b_dtype)
-        return dx, dw, db, None
-
-
 def mx_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
               checkpoint: str = "int8") -> torch.Tensor:
     """A linear layer that computes in microscaled 4-bit numbers and keeps its activations in 8 bits (or 4).
@@ -87,7 +59,7 @@ def mx_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     byte a value with ``"int8"``, or the forward's own ``q(x)`` at half a byte with ``"fp4"``.  Neither ``x`` nor
     ``weight`` is kept.  fp32, fp16 or bf16 CUDA tensors; the three may differ in type.
 
-    A backward pass can be captured into a CUDA graph, as long as no eager autograd graph of the same leaves is still
+    It can be differentiated once.  A backward pass can be captured into a CUDA graph, as long as no eager autograd graph of the same leaves is still
     alive: PyTorch would synchronise with that graph's stream, which invalidates the capture.
     """
-    return _MXLinear.apply(x, weight, bias, ops._mx_format(checkpoint))
+    return _lib.host().mx_layer(x, weight, bias, ops._mx_format(checkpoint))

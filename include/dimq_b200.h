@@ -391,6 +391,10 @@ DIMQ_API int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w_c
 DIMQ_API int dimq_mx_grad_weight(const void* dy, int dy_dtype, const void* x_codes, const uint8_t* x_scales, int format, void* dw,
                                  int dw_dtype, void* db, int db_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
                                  int64_t workspace_bytes, void* stream);
+/* dx, dw and db of one layer (each may be NULL, not all): the terms of a dy that is not bf16 are made once for both. */
+DIMQ_API int dimq_mx_grads(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, const void* x_codes,
+                           const uint8_t* x_scales, int format, void* dx, int dx_dtype, void* dw, int dw_dtype, void* db,
+                           int db_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- dense helper of the whole-model harness --------------------------- */
 
