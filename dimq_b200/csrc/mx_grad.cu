@@ -54,10 +54,25 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_box(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
+  if (PAIR) tma_load_3d_pair(dst, tmap, bar, c0, c1, c2);
+  else tma_load_3d(dst, tmap, bar, c0, c1, c2);
+}
+template <bool PAIR>
 __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // Columns contiguous: pieces of 64 columns x 8 rows of the reduction (1024 bytes, 128-byte swizzle), the next eight rows
 // 1024 bytes on, the next 64 columns a whole box (64 rows) on.
@@ -85,10 +100,12 @@ __device__ __forceinline__ Unit unit_of(int u, int steps, const GradParams& p) {
   return w;
 }
 
-template <int BN, int ES, bool SEG>
+// SEG: fp32 results of long sums, added up in registers.  PAIR: two blocks share a tile of 256 rows (BN = 256).
+template <int BN, int ES, bool SEG, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
-  constexpr uint32_t kStageBytes = kABytes + BN * kDepth * 2;
+  constexpr int kCols = PAIR ? BN / 2 : BN;      // columns of the tile that this block holds
+  constexpr uint32_t kStageBytes = kABytes + kCols * kDepth * 2;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t n_st = static_cast<uint32_t>(p.stages);
@@ -96,10 +113,13 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
   unsigned char* staging = reinterpret_cast<unsigned char*>(hdr) + kHeaderBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int all_steps = p.depth_blocks * p.terms, units = p.n_tiles * p.m_tiles * p.slices;
+  const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
+  const int unit0 = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int unit_step = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), PAIR ? 2 : 1); }
     hdr->abort_flag = 0u;
     fence_barrier_init();
     prefetch_tensormap(&maps.a);
@@ -107,12 +127,13 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     if (p.out.tma) prefetch_tensormap(&maps.y);
   }
   if (warp == kProducers) {
-    tmem_alloc(smem_u32(&hdr->tmem_base), 512);
-    tmem_relinquish();
+    if constexpr (PAIR) tmem_alloc_pair(smem_u32(&hdr->tmem_base), 512);
+    else { tmem_alloc(smem_u32(&hdr->tmem_base), 512); tmem_relinquish(); }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if constexpr (PAIR) { cluster_arrive(); cluster_wait(); }   // the peer's barriers are there before anything signals them
   const uint32_t tmem = hdr->tmem_base;
   volatile uint32_t* abort_flag = &hdr->abort_flag;
   wait_for_inputs();
@@ -122,23 +143,24 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     const uint32_t turns = n_st < kProducers ? n_st : kProducers;
     uint32_t stage = 0, phase = 0, turn = 0, issued = 0;
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    for (int u = unit0; u < units && ok; u += unit_step) {
       const Unit w = unit_of(u, all_steps, p);
-      const int n_blk = w.tile % p.n_tiles, m_blk = w.tile / p.n_tiles;
+      const int n_blk = w.tile % p.n_tiles, m_blk = (PAIR ? 2 : 1) * (w.tile / p.n_tiles) + rank;
       int term = p.terms - 1 - w.first / p.depth_blocks, kb = w.first % p.depth_blocks;   // smallest terms first
       for (int s = w.first; s < w.end; ++s) {
         if (turn == static_cast<uint32_t>(warp)) {
           if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase ^ 1u, abort_flag, 0x3100u | stage))) { ok = false; break; }
           const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * kStageBytes);
-          if (elect_one()) {
-            mbar_arrive_expect_tx(full, kStageBytes);
+          if (elect_one()) {     // a pair counts both blocks' bytes in the first one's barrier
+            if (rank == 0) mbar_arrive_expect_tx(full, (PAIR ? 2 : 1) * kStageBytes);
+            const uint32_t bar = PAIR ? map_to_cta(full, 0) : full;
             if (p.a_cols) {
-              tma_load_3d(dst, &maps.a, full, m_blk * 128, kb * kDepth, term);
-              tma_load_3d(dst + kABytes / 2, &maps.a, full, m_blk * 128 + 64, kb * kDepth, term);
+              load_box<PAIR>(dst, &maps.a, bar, m_blk * 128, kb * kDepth, term);
+              load_box<PAIR>(dst + kABytes / 2, &maps.a, bar, m_blk * 128 + 64, kb * kDepth, term);
             } else {
-              tma_load_3d(dst, &maps.a, full, kb * kDepth, m_blk * 128, term);
+              load_box<PAIR>(dst, &maps.a, bar, kb * kDepth, m_blk * 128, term);
             }
-            tma_load_3d(dst + kABytes, &maps.b, full, 0, kb * kDepth, n_blk * (BN / 64));
+            load_box<PAIR>(dst + kABytes, &maps.b, bar, 0, kb * kDepth, n_blk * (BN / 64) + rank * (kCols / 64));
           }
           __syncwarp();
         }
@@ -160,10 +182,10 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     __syncwarp();
   } else if (warp == kProducers) {
     uint32_t stage = 0, phase = 0, buf = 0, bph = 0;
-    bool ok = true;
-    const uint32_t idesc = make_idesc_f16(1, 1, 128, BN) | (p.a_cols ? 1u << 15 : 0u) | (1u << 16);
+    bool ok = rank == 0;      // the first block of a pair issues for both
+    const uint32_t idesc = make_idesc_f16(1, 1, PAIR ? 256 : 128, BN) | (p.a_cols ? 1u << 15 : 0u) | (1u << 16);
     const uint64_t a_step = p.a_cols ? 2048 >> 4 : 32 >> 4;   // 16 of the reduction
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    for (int u = unit0; u < units && ok; u += unit_step) {
       const Unit w = unit_of(u, all_steps, p);
       for (int seg0 = w.first; seg0 < w.end && ok; seg0 += SEG ? kSegStages : all_steps) {
         const int seg1 = SEG && seg0 + kSegStages < w.end ? seg0 + kSegStages : w.end;
@@ -178,14 +200,14 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
           if (elect_one()) {
 #pragma unroll
             for (int j = 0; j < kDepth / 16; ++j)
-              mma_bf16(d, a0 + a_step * j, b0 + static_cast<uint64_t>((2048 >> 4) * j), idesc, (s > seg0 || j) ? 1u : 0u);
-            mma_commit(smem_u32(&hdr->empty[stage]));
+              mma_bf16<PAIR>(d, a0 + a_step * j, b0 + static_cast<uint64_t>((2048 >> 4) * j), idesc, (s > seg0 || j) ? 1u : 0u);
+            commit<PAIR>(smem_u32(&hdr->empty[stage]));
           }
           __syncwarp();
           if (++stage == n_st) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        if (elect_one()) mma_commit(smem_u32(&hdr->d_full[buf]));
+        if (elect_one()) commit<PAIR>(smem_u32(&hdr->d_full[buf]));
         __syncwarp();
         if (++buf == 2) { buf = 0; bph ^= 1u; }
       }
@@ -198,9 +220,9 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     uint32_t buf = 0, bph = 0, piece = 0;
     bool ok = true;
     Out out = p.out;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    for (int u = unit0; u < units && ok; u += unit_step) {
       const Unit w = unit_of(u, all_steps, p);
-      const int64_t n_first = static_cast<int64_t>(w.tile % p.n_tiles) * BN, tile_row0 = static_cast<int64_t>(w.tile / p.n_tiles) * 128 + quarter * 32;
+      const int64_t n_first = static_cast<int64_t>(w.tile % p.n_tiles) * BN, tile_row0 = (static_cast<int64_t>(PAIR ? 2 : 1) * (w.tile / p.n_tiles) + rank) * 128 + quarter * 32;
       // partial results lie one under the other: a slice's rows start at slice * rows.  Only whole pieces of 32 rows go
       // through the map; a piece that ends in the next slice's rows is stored plainly.
       const int64_t row_off = static_cast<int64_t>(w.slice) * p.out.rows, row0 = tile_row0 + row_off;
@@ -233,7 +255,10 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
           if (i == kMine - 1) {
             tc_fence_before();
             bar_sync(1, kEpiWarps * 32);
-            if (ew == 0 && lane == 0) mbar_arrive(smem_u32(&hdr->d_empty[buf]));
+            if (ew == 0 && lane == 0) {
+              if constexpr (PAIR) remote_arrive(map_to_cta(smem_u32(&hdr->d_empty[buf]), 0));
+              else mbar_arrive(smem_u32(&hdr->d_empty[buf]));
+            }
           }
           __syncwarp();
           if constexpr (!SEG) {
@@ -259,9 +284,11 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) { cluster_arrive(); cluster_wait(); }   // neither block leaves while the other may use its memories
   if (warp == kProducers) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
@@ -401,18 +428,18 @@ int split_terms(const void* dy, int dtype, int64_t M, int64_t N, void* scratch, 
   return launch_status();
 }
 
-template <int BN, int ES, bool SEG>
+template <int BN, int ES, bool SEG, bool PAIR>
 int launch_grad(GradMaps& maps, GradParams& p, cudaStream_t st) {
-  constexpr size_t kStageBytes = kABytes + BN * kDepth * 2;
+  constexpr size_t kRing = kABytes + (PAIR ? BN / 2 : BN) * kDepth * 2;
   const size_t fixed = 1024 + kHeaderBytes + kEpiWarps * kStagingBytes;
-  p.stages = static_cast<int>((kSmemMax - fixed) / kStageBytes);
+  p.stages = static_cast<int>((kSmemMax - fixed) / kRing);
   if (p.stages > kMaxStages) p.stages = kMaxStages;
-  auto kern = mx_grad_kernel<BN, ES, SEG>;
+  auto kern = mx_grad_kernel<BN, ES, SEG, PAIR>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
   if (e != cudaSuccess) return static_cast<int>(e);
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.slices;
-  const unsigned grid = static_cast<unsigned>(tiles < kNumSMs ? tiles : kNumSMs);
-  e = launch_dependent(kern, grid, kThreads, fixed + p.stages * kStageBytes, st, 1, maps, p);
+  const int64_t units = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.slices, most = PAIR ? kNumSMs / 2 : kNumSMs;
+  const unsigned grid = static_cast<unsigned>((units < most ? units : most) * (PAIR ? 2 : 1));
+  e = launch_dependent(kern, grid, kThreads, fixed + p.stages * kRing, st, PAIR ? 2 : 1, maps, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
@@ -421,21 +448,22 @@ int launch_grad(GradMaps& maps, GradParams& p, cudaStream_t st) {
 // (about 3 KB a cycle over the whole chip, and a launch).  25216 tokens, 2304 x 768 weights: 54 tiles of 256 columns,
 // REPLACE us whole, REPLACE us in slices.
 struct GradPlan {
-  int bn, slices;
+  int bn, slices;     // bn 512: pairs of blocks, 256 x 256
 };
 GradPlan plan_of(int64_t R, int64_t K, int64_t depth, int terms) {
-  const int width[3] = {256, 128, 64};
-  const double cost[3] = {750.0, 520.0, 430.0};
+  const int form[4] = {512, 256, 128, 64};
+  const double cost[4] = {650.0, 750.0, 520.0, 430.0};
   const int64_t steps = (depth + kDepth - 1) / kDepth * terms;
-  GradPlan best = {256, 1};
+  GradPlan best = {512, 1};
   double least = -1.0;
-  for (int i = 0; i < 3; ++i) {
-    const int64_t tiles = row_tiles(R) * ((K + width[i] - 1) / width[i]);
-    for (int s = 1; s <= 16 && (s == 1 || (s * kSegStages <= steps && tiles * (s - 1) < kNumSMs)); ++s) {
-      const double waves = static_cast<double>((tiles * s + kNumSMs - 1) / kNumSMs);
+  for (int i = 0; i < 4; ++i) {
+    const int64_t width = form[i] > 256 ? 256 : form[i], side_by_side = form[i] > 256 ? kNumSMs / 2 : kNumSMs;
+    const int64_t tiles = (form[i] > 256 ? (row_tiles(R) + 1) / 2 : row_tiles(R)) * ((K + width - 1) / width);
+    for (int s = 1; s <= 16 && (s == 1 || (s * kSegStages <= steps && tiles * (s - 1) < side_by_side)); ++s) {
+      const double waves = static_cast<double>((tiles * s + side_by_side - 1) / side_by_side);
       double c = waves * (static_cast<double>((steps + s - 1) / s) * cost[i] + 2000.0);
       if (s > 1) c += 6000.0 + static_cast<double>(R) * K * 8 * s / 3000.0;
-      if (least < 0.0 || c < least) { least = c; best = {width[i], s}; }
+      if (least < 0.0 || c < least) { least = c; best = {form[i], s}; }
     }
   }
   return best;
@@ -451,7 +479,8 @@ int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms,
   GradMaps maps;
   GradParams p = {};
   const GradPlan plan = plan_of(out.rows, K, depth, terms);
-  const int bn = plan.bn;
+  const bool pair = plan.bn > 256;
+  const int bn = pair ? 256 : plan.bn;
   const Out result = out;
   if (plan.slices > 1) {
     out.y = partial;
@@ -463,7 +492,7 @@ int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms,
   p.slices = plan.slices;
   p.a_cols = a_cols;
   p.depth_blocks = static_cast<int>((depth + kDepth - 1) / kDepth);
-  const int64_t n_tiles = (K + bn - 1) / bn, m_tiles = row_tiles(out.rows);
+  const int64_t n_tiles = (K + bn - 1) / bn, m_tiles = pair ? (row_tiles(out.rows) + 1) / 2 : row_tiles(out.rows);
   if (n_tiles * m_tiles * plan.slices > 0x7FFFFFFF - kNumSMs || static_cast<int64_t>(p.depth_blocks) * terms > 0x7FFFFFFF - 64 ||
       out.rows * plan.slices > 0x7FFFFF00)
     return DIMQ_ERR_TOO_LARGE;
@@ -475,7 +504,7 @@ int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms,
   const cuuint32_t abox[3] = {64, a_cols ? 64u : 128u, 1};
   const cuuint64_t bdims[3] = {64, static_cast<cuuint64_t>(depth), static_cast<cuuint64_t>(up(K, 64) / 64)};
   const cuuint64_t bstr[2] = {128, static_cast<cuuint64_t>(depth) * 128};
-  const cuuint32_t bbox[3] = {64, kDepth, static_cast<cuuint32_t>(bn / 64)};
+  const cuuint32_t bbox[3] = {64, kDepth, static_cast<cuuint32_t>((pair ? bn / 2 : bn) / 64)};
   Out rows_of_all = out;
   rows_of_all.rows *= plan.slices;
   if (!encode_map(&maps.a, bf16, 3, dy, adims, astr, abox, CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -484,9 +513,10 @@ int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms,
     return DIMQ_ERR_DRIVER;
   const bool wide = result.dtype == DIMQ_F32, seg = wide && p.depth_blocks * terms > kSegStages * plan.slices;
   int rc;
-#define DIMQ_MX_GRAD(ES, SEG)                                   \
-  rc = bn == 256 ? launch_grad<256, ES, SEG>(maps, p, st)       \
-       : bn == 128 ? launch_grad<128, ES, SEG>(maps, p, st) : launch_grad<64, ES, SEG>(maps, p, st)
+#define DIMQ_MX_GRAD(ES, SEG)                                          \
+  rc = pair ? launch_grad<256, ES, SEG, true>(maps, p, st)             \
+       : bn == 256 ? launch_grad<256, ES, SEG, false>(maps, p, st)     \
+       : bn == 128 ? launch_grad<128, ES, SEG, false>(maps, p, st) : launch_grad<64, ES, SEG, false>(maps, p, st)
   if (seg) { DIMQ_MX_GRAD(4, true); }
   else if (out.dtype == DIMQ_F32) { DIMQ_MX_GRAD(4, false); }
   else { DIMQ_MX_GRAD(2, false); }
