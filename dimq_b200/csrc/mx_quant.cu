@@ -25,7 +25,7 @@ __device__ __forceinline__ uint32_t gather_bytes(uint32_t b, int lane) {
 
 // C4 / C8: the formats written
 template <typename T, bool VEC, bool C4, bool C8>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && VEC ? 6 : 1)   // 42 registers: 11008 x 4096 bf16 25 -> 22 us (fp32: slower)
 mx_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t spans, uint8_t* __restrict__ codes4,
                    uint8_t* __restrict__ scales4, uint8_t* __restrict__ codes8, uint8_t* __restrict__ scales8) {
   __shared__ __align__(16) unsigned char swap[VEC ? 16 : 8 * kSpan * sizeof(T)];
@@ -102,7 +102,7 @@ __device__ __forceinline__ Eight<__nv_bfloat16> pack_values<__nv_bfloat16>(const
 // Without PANELS out is [rows][cols].  With them it is [columns / 64][rows][64], zeros behind the last column: what TMA
 // takes as boxes of 64 columns.  fill: columns written (cols, or the panels' 64s).
 template <typename T, bool VEC, bool FP4, bool PANELS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, VEC && !FP4 ? 6 : 1)              // 8192 x 4096 int8 19 -> 17 us (fp4: no gain)
 mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
                      int64_t spans, T* __restrict__ out, int64_t fill) {
   __shared__ __align__(16) unsigned char swap[VEC ? 16 : 8 * kSpan * sizeof(T)];
@@ -144,7 +144,21 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
       }
     }
     const Eight<T> e = pack_values<T>(v);
-    if constexpr (VEC) {
+    if constexpr (VEC && sizeof(T) == 4) {
+      // two lanes exchange halves, so that each store of the warp writes whole sectors: the 32 bytes of the even lanes'
+      // values, then those of the odd lanes'
+      const bool odd = lane & 1;
+      uint32_t mine[4], theirs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        theirs[i] = __shfl_xor_sync(0xFFFFFFFFu, odd ? e.w[i] : e.w[4 + i], 1);
+        mine[i] = odd ? e.w[4 + i] : e.w[i];
+      }
+      const int64_t base = k - (odd ? 8 : 0) + (odd ? 4 : 0);   // even lane: its first half; odd lane: the even lane's second
+      T* dst = out + row * cols;
+      if (base < fill) *reinterpret_cast<uint4*>(dst + base) = odd ? make_uint4(theirs[0], theirs[1], theirs[2], theirs[3]) : make_uint4(mine[0], mine[1], mine[2], mine[3]);
+      if (base + 8 < fill) *reinterpret_cast<uint4*>(dst + base + 8) = odd ? make_uint4(mine[0], mine[1], mine[2], mine[3]) : make_uint4(theirs[0], theirs[1], theirs[2], theirs[3]);
+    } else if constexpr (VEC) {
       T* dst = PANELS ? out + ((k >> 6) * rows + row) * 64 + (k & 63) : out + row * cols + k;
       constexpr int kPer = 16 / sizeof(T);
 #pragma unroll

@@ -256,13 +256,29 @@ int launch_small(const CUtensorMap& codes, SmallParams p, bool vec, int64_t row_
 template <typename T>
 int small_as(const CUtensorMap& codes, const SmallParams& p, bool vec, int64_t row_blocks, cudaStream_t st) {
   if (p.out.rows <= 8) return launch_small<8, T>(codes, p, vec, row_blocks, st);
-  return launch_small<16, T>(codes, p, vec, row_blocks, st);
+  if (p.out.rows <= 16) return launch_small<16, T>(codes, p, vec, row_blocks, st);
+  return launch_small<32, T>(codes, p, vec, row_blocks, st);
 }
 
 }  // namespace
 
+// Blocks of a cluster: as many as let the grid run side by side, three blocks to an SM
+static int slices_of(int64_t row_blocks, int steps) {
+  int slices = 1;
+  while (slices < kMostSlices && 2 * slices <= steps &&
+         (row_blocks * slices * 2 <= 3 * kNumSMs || (steps + slices - 1) / slices > kMostSteps))
+    slices *= 2;
+  return slices;
+}
+
+// Up to 16 rows always; up to 32 where a block's slice of x is short (1024 k): every block quantises its slice, so long
+// ones cost more than a second launch (32 x 4096 -> 4096 8.3 us against 12.4, 32 x 8192 -> 8192 20.4 against 17.3).
 bool mx_small_takes(int64_t M, int64_t N, int64_t K) {
-  return M <= 16 && (mx::block_tiles(K) + 1) / 2 <= kMostSteps * kMostSlices && mx::row_tiles(N) <= 0x7FFFFFFF / kMostSlices;
+  if (M > 32) return false;
+  const int64_t steps = (mx::block_tiles(K) + 1) / 2, row_blocks = mx::row_tiles(N);
+  if (steps > kMostSteps * kMostSlices || row_blocks > 0x7FFFFFFF / kMostSlices) return false;
+  const int slices = slices_of(row_blocks, static_cast<int>(steps));
+  return M <= 16 || (steps + slices - 1) / slices <= 4;
 }
 
 int mx_small(const void* x, int x_dtype, const uint8_t* wc, const uint8_t* ws, const void* bias, int bias_dtype, const void* residual,
@@ -275,11 +291,7 @@ int mx_small(const void* x, int x_dtype, const uint8_t* wc, const uint8_t* ws, c
   p.k_tiles = static_cast<int>(block_tiles(K));
   p.steps = (p.k_tiles + 1) / 2;
   const int64_t row_blocks = row_tiles(N);
-  // as many blocks as run side by side, three to an SM
-  int slices = 1;
-  while (slices < kMostSlices && 2 * slices <= p.steps &&
-         (row_blocks * slices * 2 <= 3 * kNumSMs || (p.steps + slices - 1) / slices > kMostSteps))
-    slices *= 2;
+  const int slices = slices_of(row_blocks, p.steps);
   p.slices = slices;
   p.room = (p.steps + slices - 1) / slices;
   CUtensorMap codes;

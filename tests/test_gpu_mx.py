@@ -134,7 +134,7 @@ def _check_linear(y, x4, w4, bias, epilogue, residual, out_dtype):
     _mx.check(y.reshape(rows, -1), want, bound.nan_to_num() + _mx.rounding(want.nan_to_num() + bound.nan_to_num(), out_dtype), "y")
 
 
-LINEAR = [(1, 1, 1), (1, 32, 8), (3, 33, 7), (2, 100, 128), (8, 256, 130), (16, 1000, 129), (17, 1024, 64), (1, 4096, 256), (5, 8320, 128),
+LINEAR = [(1, 1, 1), (1, 32, 8), (3, 33, 7), (2, 100, 128), (8, 256, 130), (16, 1000, 129), (17, 1024, 64), (32, 16500, 136), (27, 4100, 300), (1, 4096, 256), (5, 8320, 128),
           (33, 520, 257), (64, 2050, 100), (128, 128, 128), (130, 300, 257), (197, 768, 96), (300, 1001, 515), (257, 512, 640),
           (16, 16500, 130), (5, 32768, 40), (3, 33000, 40), (2500, 330, 2568), (1300, 4420, 2600)]
 
@@ -207,7 +207,7 @@ def test_linear_leading_dimensions_strides_empty(cuda_device):
     assert torch.equal(ops.mx_linear(x, codes, scales, bias, 40, 96), ops.mx_linear(x, codes, scales, bias.clone(), 40, 96))
 
 
-@pytest.mark.parametrize("m", [1, 16, 17, 128, 500])
+@pytest.mark.parametrize("m", [1, 16, 17, 32, 33, 128, 500])
 def test_linear_rows_do_not_depend_on_their_neighbours(cuda_device, m):
     """A row's result is the same bits twice, and does not change with the values of the other rows."""
     from dimq_b200 import ops
