@@ -219,25 +219,30 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
       const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
       float sum[kMine][32];
       for (int seg0 = 0; seg0 < k_stages; seg0 += SEG ? kSegStages : k_stages) {
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf))) { ok = false; break; }
-        tc_fence_after();
-        // all of this warp's sums into registers: the accumulator is free before they are looked at
-        if constexpr (SEG) {
+        const bool there = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf));
+        if (there) {
+          tc_fence_after();
+          // all of this warp's sums into registers: the accumulator is free before they are looked at
+          if constexpr (SEG) {
 #pragma unroll
-          for (int i = 0; i < kMine; ++i) {
-            uint32_t r[32];
-            tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, r);
+            for (int i = 0; i < kMine; ++i) {
+              uint32_t r[32];
+              tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sum[i][j] = seg0 == 0 ? __uint_as_float(r[j]) : sum[i][j] + __uint_as_float(r[j]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, reinterpret_cast<uint32_t(&)[32]>(sum[i]));
             tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) sum[i][j] = seg0 == 0 ? __uint_as_float(r[j]) : sum[i][j] + __uint_as_float(r[j]);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kMine; ++i) tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, reinterpret_cast<uint32_t(&)[32]>(sum[i]));
-          tmem_ld_wait();
+          tc_fence_before();
         }
-        tc_fence_before();
-        bar_sync(1, kEpiWarps * 32);      // one arrival for all: sixteen, half of them from the other block, held 18944 x 256 -> 2048 at 30 us (24)
+        // The warps meet, whether they got there or not (all leave together), and one arrival stands for all: sixteen on one
+        // barrier, half of them from the other block, held 18944 x 256 -> 2048 at 30 us (24).
+        ok = all_agree(1, kEpiWarps * 32, there);
+        if (!ok) break;
         if (ew == 0 && lane == 0) {
           if constexpr (PAIR) remote_arrive(map_to_cta(smem_u32(&hdr->d_empty[buf]), 0));
           else mbar_arrive(smem_u32(&hdr->d_empty[buf]));

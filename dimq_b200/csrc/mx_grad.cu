@@ -46,7 +46,7 @@ struct GradParams {
 
 struct GradHeader {
   uint64_t full[kMaxStages], empty[kMaxStages], d_full[2], d_empty[2];
-  uint32_t tmem_base;
+  uint32_t tmem_base, drained[2];
   volatile uint32_t abort_flag;
 };
 
@@ -121,6 +121,7 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), PAIR ? 2 : 1); }
     hdr->abort_flag = 0u;
+    hdr->drained[0] = hdr->drained[1] = 0u;
     fence_barrier_init();
     prefetch_tensormap(&maps.a);
     prefetch_tensormap(&maps.b);
@@ -254,11 +255,8 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
           }
           if (i == kMine - 1) {
             tc_fence_before();
-            bar_sync(1, kEpiWarps * 32);
-            if (ew == 0 && lane == 0) {
-              if constexpr (PAIR) remote_arrive(map_to_cta(smem_u32(&hdr->d_empty[buf]), 0));
-              else mbar_arrive(smem_u32(&hdr->d_empty[buf]));
-            }
+            __syncwarp();
+            if (lane == 0) hand_back<PAIR>(&hdr->drained[buf], smem_u32(&hdr->d_empty[buf]));
           }
           __syncwarp();
           if constexpr (!SEG) {

@@ -191,6 +191,7 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
     }
   }
   tc_fence_before();
+  __syncwarp();             // the cluster's barrier wants whole warps
   if (slices > 1) {
     cluster_arrive();
     cluster_wait();
@@ -223,6 +224,7 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
     const float res = p.out.residual != nullptr ? load_as_float(p.out.residual, p.out.dtype, o) : 0.0f;
     store_from_float(p.out.y, p.out.dtype, o, activate_any(s, res, p.out.epilogue));
   }
+  __syncwarp();
   if (slices > 1) {         // no block leaves while a peer may read its sums
     cluster_arrive();
     cluster_wait();

@@ -146,6 +146,28 @@ __device__ __forceinline__ void commit(uint32_t bar) {   // PAIR: one arrival in
     mma_commit(bar);
 }
 
+// One lane of an epilogue warp whose sums are in registers: the last of the warps hands the accumulator back (PAIR: to the
+// first block's barrier).  Nothing waits here: with two accumulators the warps need not keep step (a barrier among them held
+// the fp32 8192 x 11008 -> 4096 weight gradient at 630 us, 540 so).
+template <bool PAIR>
+__device__ __forceinline__ void hand_back(uint32_t* count, uint32_t bar) {
+  __threadfence_block();
+  if (atomicAdd(count, 1u) == kEpiWarps - 1) {
+    *count = 0u;
+    __threadfence_block();
+    if (PAIR) remote_arrive(map_to_cta(bar, 0));
+    else mbar_arrive(bar);
+  }
+}
+
+// Whether all of a barrier's `threads` (whole warps) say yes
+__device__ __forceinline__ bool all_agree(int id, int threads, bool yes) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"(static_cast<uint32_t>(yes)), "r"(id), "r"(threads) : "memory");
+  return r != 0u;
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays one
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
