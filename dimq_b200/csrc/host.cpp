@@ -807,7 +807,6 @@ Mx mx_quantize(const Tensor& x, int format, int* launches) {
 }
 
 const uint8_t* bytes_of(const Tensor& t) { return static_cast<const uint8_t*>(t.data_ptr()); }
-uint8_t* writable(Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
 Tensor mx_dequantize(const Tensor& codes, const Tensor& scales, int64_t cols, int format, at::ScalarType dt, int* launches) {
   int64_t rows = -1;
@@ -819,19 +818,6 @@ Tensor mx_dequantize(const Tensor& codes, const Tensor& scales, int64_t cols, in
                            stream_of(codes)), "mx_dequantize");
   *launches = rows > 0;
   return y;
-}
-
-// x: values, or (x_scales) the codes of a 4-bit quantisation
-void mx_linear_into(const Tensor& x, int xd, const OptTensor& x_scales, const Mx& w, const Bias& b, const OptTensor& res, Tensor& y,
-                    int64_t m, int64_t n, int64_t k, int epilogue, int* launches) {
-  int64_t need = 0;
-  check(dimq_mx_linear_workspace_bytes(m, n, k, x_scales.has_value(), &need), "mx_linear_workspace_bytes");
-  OptTensor ws;
-  if (need > 0 && m > 0) ws = scratch(need, x);
-  check(dimq_mx_linear(x.data_ptr(), xd, x_scales.has_value() ? bytes_of(*x_scales) : nullptr, bytes_of(w.codes), bytes_of(w.scales),
-                       ptr(b.t), b.dtype, ptr(res), y.data_ptr(), dtype_code(y, "y"), m, n, k, epilogue,
-                       ws.has_value() ? ws->data_ptr() : nullptr, need, stream_of(x)), "mx_linear");
-  *launches += m > 0 ? 1 + (need > 0) : 0;
 }
 
 Tensor mx_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& bias, int64_t n, int64_t k,
@@ -848,7 +834,14 @@ Tensor mx_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, con
   const Tensor xc = x.contiguous();
   Tensor y = at::empty(out_shape(x, n), x.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
   const OptTensor res = linear_residual(residual, y);
-  mx_linear_into(xc, xd, std::nullopt, w, b, res, y, mx_rows(x, k), n, k, epilogue, launches);
+  const int64_t m = mx_rows(x, k);
+  int64_t need = 0;      // a few rows are quantised by the product itself
+  check(dimq_mx_linear_workspace_bytes(m, n, k, 0, &need), "mx_linear_workspace_bytes");
+  OptTensor ws;
+  if (need > 0 && m > 0) ws = scratch(need, x);
+  check(dimq_mx_linear(xc.data_ptr(), xd, nullptr, bytes_of(w.codes), bytes_of(w.scales), ptr(b.t), b.dtype, ptr(res), y.data_ptr(),
+                       dtype_code(y, "y"), m, n, k, epilogue, ws.has_value() ? ws->data_ptr() : nullptr, need, stream_of(x)), "mx_linear");
+  *launches += m > 0 ? 1 + (need > 0) : 0;
   return y;
 }
 
@@ -970,6 +963,15 @@ class MxLayer : public torch::autograd::Function<MxLayer> {
     return f.y;
   }
 
+  // A kept buffer as the backward gets it: hooks on saved tensors may have had it elsewhere in between.
+  static MxBuffer kept(const Tensor& t, const Tensor& dy, int64_t rows, int64_t cols, int format) {
+    const MxSizes s = mx_sizes(rows, cols, format);
+    const int64_t at = mx_scales_at(rows, s);
+    if (!t.defined() || t.scalar_type() != at::kByte || t.numel() != at + s.scale_bytes) fail("mx_linear: a kept activation or weight has another size or type");
+    same_device(t, dy, "what mx_linear keeps");
+    return {aligned16(t), at};
+  }
+
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const int64_t n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
@@ -990,8 +992,8 @@ class MxLayer : public torch::autograd::Function<MxLayer> {
     if (need_b) db = at::empty({n}, opt.dtype(type("b")));
     if (!need_x && !need_w && !need_b) return out;
     MxBuffer x, w;
-    if (need_w) x = {saved[0], mx_scales_at(m, mx_sizes(m, k, keep))};
-    if (need_x) w = {saved[1], mx_scales_at(n, mx_sizes(n, k, DIMQ_MX_FP4))};
+    if (need_w) x = kept(saved[0], g, m, k, keep);
+    if (need_x) w = kept(saved[1], g, n, k, DIMQ_MX_FP4);
     int64_t need = 0;
     check(dimq_mx_grad_workspace_bytes(dyd, m, n, k, &need), "mx_grad_workspace_bytes");
     const Tensor ws = scratch(need, g);

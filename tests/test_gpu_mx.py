@@ -339,6 +339,31 @@ def test_layer_only_what_is_needed(cuda_device):
         torch.autograd.grad(g.float().sum(), full[1])
 
 
+def test_layer_under_saved_tensor_hooks_and_recomputation(cuda_device):
+    """What the layer keeps may wait on the host, be computed again, or come back wrong (which is refused)."""
+    from torch.utils.checkpoint import checkpoint
+
+    from dimq_b200 import qat
+
+    leaves = [t.requires_grad_() for t in (_values(40, 96, torch.bfloat16, 17), _values(24, 96, torch.float32, 18), torch.randn(24, device="cuda"))]
+    dy = _values(40, 24, torch.bfloat16, 19)
+    want = torch.autograd.grad(qat.mx_linear(*leaves), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = qat.mx_linear(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
+    y = checkpoint(qat.mx_linear, *leaves, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
+    for spoil in (lambda t: t.cpu(), lambda t: t[:-1], lambda t: t.int()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spoil):
+            y = qat.mx_linear(*leaves)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaves, dy)
+    y = qat.mx_linear(*leaves)
+    torch.autograd.grad(y, leaves, dy)
+    with pytest.raises(RuntimeError):      # the graph is gone
+        torch.autograd.grad(y, leaves, dy)
+
+
 def test_layer_empty_batch(cuda_device):
     from dimq_b200 import qat
 

@@ -70,6 +70,12 @@ def test_argument_errors_are_reported_without_a_gpu(lib):
     assert grad_w(fmt=2) == -4 and grad_w(dyd=4) == -3 and grad_w(dwd=4) == -3 and grad_w(db=one, dbd=4) == -3
     assert grad_w(dw=null) == -1 and grad_w(dy=null) == -1 and grad_w(xc=null) == -1 and grad_w(n=0) == -2
     assert grad_w(xs=odd) == -8 and grad_w(work=null) == -12 and grad_w(size=8) == -12
+
+    def grads(dy=one, wc=one, ws=one, xc=one, xs=one, fmt=8, dx=one, dw=one, db=one, m=2, work=one, size=1 << 30):
+        return lib.dimq_mx_grads(dy, 0, wc, ws, xc, xs, fmt, dx, 0, dw, 0, db, 0, i(m), i(8), i(32), work, i(size), null)
+
+    assert grads(dx=null, dw=null, db=null) == -1 and grads(dy=null) == -1 and grads(wc=null) == -1 and grads(xs=null) == -1
+    assert grads(fmt=5) == -4 and grads(ws=odd) == -8 and grads(dy=odd) == -8 and grads(work=null) == -12 and grads(m=-1) == -2
     assert lib.dimq_mx_grad_workspace_bytes(5, i(1), i(1), i(1), C.byref(need)) == -3
     assert lib.dimq_mx_grad_workspace_bytes(0, i(1), i(1), i(1), None) == -1
 
