@@ -4,6 +4,9 @@
 // two operands' powers of two before it adds: products and scaling are exact, sums are fp32.  So nothing is decoded: TMA
 // brings codes (rows of 128 bytes = 256 values, 128-byte swizzle) and the 512-byte scale tiles that the format keeps,
 // tcgen05.cp moves a scale tile to tensor memory, and the accumulators go through bias, activation and residual to y.
+// Products are multiples of a quarter of their blocks' scales and 64 of them take one step, so the cut to fp32 at each step
+// rarely loses a bit: against 64 bits the sums of normal values are exact (K = 32768), those of blocks whose scales differ by
+// 2^12 and more are within 1.2e-7 (K = 11008) to 6.9e-7 (K = 32768).
 //
 // Large problems run on pairs of blocks (cta_group::2): 256 x 256 tiles, each block holding its 128 rows of x and half of
 // the tile's rows of w, so that a step moves 32 KB of codes into each shared memory instead of 48.  The first block of a
@@ -32,7 +35,6 @@ constexpr int kMaxStages = 8;
 constexpr int kSfCol = 256;                      // first tensor-memory column of the scales
 constexpr uint32_t kABytes = 128 * 128;
 constexpr int kBiasBytes = kEpiWarps * 4 * 128;  // four pieces of 32 columns a warp
-constexpr int kSegStages = 8;                    // fp32 results: sums of 2048 k are added up in registers
 
 struct GemmMaps {
   CUtensorMap a, b, y, sfa, sfb;   // scales: pairs only
@@ -62,8 +64,8 @@ struct Shape {
   static constexpr int kMost = (512 - kSfCol) / kSfCols < kMaxStages ? (512 - kSfCol) / kSfCols : kMaxStages;
 };
 
-// SEG: fp32 results of long sums, added up in registers (BN <= 128).  PAIR: BN = 256.
-template <int BN, int ES, bool SEG, bool PAIR>
+// PAIR: BN = 256.
+template <int BN, int ES, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
   using S = Shape<BN, PAIR>;
@@ -157,44 +159,41 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     bool ok = rank == 0;      // the first block of a pair issues for both
     for (int t = tile0; t < p.tiles && ok; t += tile_step) {
       const int n0 = (t % p.n_tiles) * BN;
-      for (int seg0 = 0; seg0 < k_stages && ok; seg0 += SEG ? kSegStages : k_stages) {
-        const int seg1 = SEG && seg0 + kSegStages < k_stages ? seg0 + kSegStages : k_stages;
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_empty[buf]), bph ^ 1u, abort_flag, 0x2200u | buf))) { ok = false; break; }
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_empty[buf]), bph ^ 1u, abort_flag, 0x2200u | buf))) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t d = tmem + buf * 128;
+      for (int kb = 0; kb < k_stages; ++kb) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->full[stage]), phase, abort_flag, 0x2300u | stage))) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d = tmem + buf * 128;
-        for (int kb = seg0; kb < seg1; ++kb) {
-          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->full[stage]), phase, abort_flag, 0x2300u | stage))) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
-          const uint64_t a0 = make_smem_desc_sw128(at), b0 = make_smem_desc_sw128(at + kABytes);
-          const uint64_t sf0 = scale_desc(at + kABytes + S::kBBytes);
-          const uint32_t sfa = tmem + kSfCol + stage * S::kSfCols, sfb = sfa + 8;
-          const int kts = p.k_tiles - 2 * kb < 2 ? p.k_tiles - 2 * kb : 2;
-          if (elect_one()) {
+        const uint32_t at = smem_u32(smem + stage * S::kStageBytes);
+        const uint64_t a0 = make_smem_desc_sw128(at), b0 = make_smem_desc_sw128(at + kABytes);
+        const uint64_t sf0 = scale_desc(at + kABytes + S::kBBytes);
+        const uint32_t sfa = tmem + kSfCol + stage * S::kSfCols, sfb = sfa + 8;
+        const int kts = p.k_tiles - 2 * kb < 2 ? p.k_tiles - 2 * kb : 2;
+        if (elect_one()) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-              if (kt < kts) {   // a scale tile that is not there has no values either
-                copy_scales<PAIR>(sfa + 4 * kt, sf0 + static_cast<uint64_t>(kt * (kTileBytes >> 4)));
+          for (int kt = 0; kt < 2; ++kt) {
+            if (kt < kts) {   // a scale tile that is not there has no values either
+              copy_scales<PAIR>(sfa + 4 * kt, sf0 + static_cast<uint64_t>(kt * (kTileBytes >> 4)));
 #pragma unroll
-                for (int i = 0; i < S::kRowTiles; ++i)
-                  copy_scales<PAIR>(sfb + (kt * S::kRowTiles + i) * 4, sf0 + static_cast<uint64_t>((1024 * (1 + i) + kt * kTileBytes) >> 4));
+              for (int i = 0; i < S::kRowTiles; ++i)
+                copy_scales<PAIR>(sfb + (kt * S::kRowTiles + i) * 4, sf0 + static_cast<uint64_t>((1024 * (1 + i) + kt * kTileBytes) >> 4));
 #pragma unroll
-                for (int j = 0; j < 2; ++j)   // 64 k = 32 bytes inside the swizzled row
-                  mma_mxf4<PAIR>(d, a0 + static_cast<uint64_t>(4 * kt + 2 * j), b0 + static_cast<uint64_t>(4 * kt + 2 * j),
-                                 mxf4_idesc(PAIR ? 256 : 128, BN, j), sfa + 4 * kt,
-                                 sfb + kt * S::kRowTiles * 4 + (BN == 64 && (n0 & 64) ? 2 : 0), (kb > seg0 || kt || j) ? 1u : 0u);
-              }
+              for (int j = 0; j < 2; ++j)   // 64 k = 32 bytes inside the swizzled row
+                mma_mxf4<PAIR>(d, a0 + static_cast<uint64_t>(4 * kt + 2 * j), b0 + static_cast<uint64_t>(4 * kt + 2 * j),
+                               mxf4_idesc(PAIR ? 256 : 128, BN, j), sfa + 4 * kt,
+                               sfb + kt * S::kRowTiles * 4 + (BN == 64 && (n0 & 64) ? 2 : 0), (kb || kt || j) ? 1u : 0u);
             }
-            commit<PAIR>(smem_u32(&hdr->empty[stage]));
           }
-          __syncwarp();
-          if (++stage == n_st) { stage = 0; phase ^= 1u; }
+          commit<PAIR>(smem_u32(&hdr->empty[stage]));
         }
-        if (!ok) break;
-        if (elect_one()) commit<PAIR>(smem_u32(&hdr->d_full[buf]));
         __syncwarp();
-        if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
+        if (++stage == n_st) { stage = 0; phase ^= 1u; }
       }
+      if (!ok) break;
+      if (elect_one()) commit<PAIR>(smem_u32(&hdr->d_full[buf]));
+      __syncwarp();
+      if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
     }
   } else {
     const int ew = warp - kProducers - 1;
@@ -218,39 +217,24 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
       }
       const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
       float sum[kMine][32];
-      for (int seg0 = 0; seg0 < k_stages; seg0 += SEG ? kSegStages : k_stages) {
-        const bool there = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf));
-        if (there) {
-          tc_fence_after();
-          // all of this warp's sums into registers: the accumulator is free before they are looked at
-          if constexpr (SEG) {
+      const bool there = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->d_full[buf]), bph, abort_flag, 0x2500u | buf));
+      if (there) {   // all of this warp's sums into registers: the accumulator is free before they are looked at
+        tc_fence_after();
 #pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-              uint32_t r[32];
-              tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) sum[i][j] = seg0 == 0 ? __uint_as_float(r[j]) : sum[i][j] + __uint_as_float(r[j]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, reinterpret_cast<uint32_t(&)[32]>(sum[i]));
-            tmem_ld_wait();
-          }
-          tc_fence_before();
-        }
-        // The warps meet, whether they got there or not (all leave together), and one arrival stands for all: sixteen on one
-        // barrier, half of them from the other block, held 18944 x 256 -> 2048 at 30 us (24).
-        ok = all_agree(1, kEpiWarps * 32, there);
-        if (!ok) break;
-        if (ew == 0 && lane == 0) {
-          if constexpr (PAIR) remote_arrive(map_to_cta(smem_u32(&hdr->d_empty[buf]), 0));
-          else mbar_arrive(smem_u32(&hdr->d_empty[buf]));
-        }
-        __syncwarp();
-        if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
+        for (int i = 0; i < kMine; ++i) tmem_ld32(tmem + lanes + buf * 128 + (sub + 2 * i) * 32, reinterpret_cast<uint32_t(&)[32]>(sum[i]));
+        tmem_ld_wait();
+        tc_fence_before();
       }
+      // The warps meet, whether they got there or not (all leave together), and one arrival stands for all: sixteen on one
+      // barrier, half of them from the other block, held 18944 x 256 -> 2048 at 30 us (24).
+      ok = all_agree(1, kEpiWarps * 32, there);
       if (!ok) break;
+      if (ew == 0 && lane == 0) {
+        if constexpr (PAIR) remote_arrive(map_to_cta(smem_u32(&hdr->d_empty[buf]), 0));
+        else mbar_arrive(smem_u32(&hdr->d_empty[buf]));
+      }
+      __syncwarp();
+      if (++buf == S::kBufs) { buf = 0; bph ^= 1u; }
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const int64_t n0 = n_first + (sub + 2 * i) * 32;
@@ -281,7 +265,7 @@ bool scale_map(CUtensorMap* m, const uint8_t* scales, int64_t rows, int64_t K, i
   return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, scales, dims, &pitch, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <int BN, int ES, bool SEG, bool PAIR>
+template <int BN, int ES, bool PAIR>
 int launch_gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& out, int64_t K, cudaStream_t st) {
   using S = Shape<BN, PAIR>;
   GemmMaps maps;
@@ -302,7 +286,7 @@ int launch_gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const u
   const size_t fixed = 1024 + kHeaderBytes + kBiasBytes + kEpiWarps * kStagingBytes;
   p.stages = static_cast<int>((kSmemMax - fixed) / S::kStageBytes);
   if (p.stages > S::kMost) p.stages = S::kMost;
-  auto kern = mx_gemm_kernel<BN, ES, SEG, PAIR>;
+  auto kern = mx_gemm_kernel<BN, ES, PAIR>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax));
   if (e != cudaSuccess) return static_cast<int>(e);
   const int64_t most = PAIR ? kNumSMs / 2 : kNumSMs;
@@ -329,20 +313,14 @@ int choose_bn(int64_t M, int64_t N) {
 }
 
 int gemm(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& out, int64_t K, cudaStream_t st) {
-  const bool wide = out.dtype == DIMQ_F32, seg = wide && block_tiles(K) > 2 * kSegStages;
   const int bn = choose_bn(out.rows, out.cols);
-#define DIMQ_MX_GEMM(BN, ES, SEG, PAIR) return launch_gemm<BN, ES, SEG, PAIR>(xc, xs, wc, ws, out, K, st)
-  if (seg) { if (bn == 64) DIMQ_MX_GEMM(64, 4, true, false); DIMQ_MX_GEMM(128, 4, true, false); }
-  if (wide) {
-    if (bn == 512) DIMQ_MX_GEMM(256, 4, false, true);
-    if (bn == 256) DIMQ_MX_GEMM(256, 4, false, false);
-    if (bn == 128) DIMQ_MX_GEMM(128, 4, false, false);
-    DIMQ_MX_GEMM(64, 4, false, false);
-  }
-  if (bn == 512) DIMQ_MX_GEMM(256, 2, false, true);
-  if (bn == 256) DIMQ_MX_GEMM(256, 2, false, false);
-  if (bn == 128) DIMQ_MX_GEMM(128, 2, false, false);
-  DIMQ_MX_GEMM(64, 2, false, false);
+#define DIMQ_MX_GEMM(BN, PAIR)                                                                \
+  return out.dtype == DIMQ_F32 ? launch_gemm<BN, 4, PAIR>(xc, xs, wc, ws, out, K, st)         \
+                               : launch_gemm<BN, 2, PAIR>(xc, xs, wc, ws, out, K, st)
+  if (bn == 512) DIMQ_MX_GEMM(256, true);
+  if (bn == 256) DIMQ_MX_GEMM(256, false);
+  if (bn == 128) DIMQ_MX_GEMM(128, false);
+  DIMQ_MX_GEMM(64, false);
 #undef DIMQ_MX_GEMM
 }
 

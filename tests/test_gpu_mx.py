@@ -522,6 +522,32 @@ def test_threads_and_streams(cuda_device):
     assert not errors, errors
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """2.3e9 values: the last rows and columns are what they are in a call of their own."""
+    from dimq_b200 import ops
+
+    m, n, k = 70001, 32776, 64
+    x, w = _values(m, k, torch.bfloat16, 50, 0.5), _values(n, k, torch.float32, 51, 0.5)
+    wq = ops.mx_quantize(w)
+    y = ops.mx_linear(x, *wq, None, n, k, out_dtype=torch.bfloat16)
+    assert torch.equal(y[-3:], ops.mx_linear(x[-3:], *wq, None, n, k, out_dtype=torch.bfloat16))       # 64 terms of few bits: exact sums
+    kept = ops.mx_quantize(x, "int8")
+    dx, dw = ops.mx_linear_grad_input(y, *wq, k), ops.mx_linear_grad_weight(y, *kept, k)
+    last = y[-3:].cpu().double()
+    w4, x8 = _mx.quantize64(w, "fp4")[2], _mx.quantize64(x, "int8")[2]
+    _mx.check(dx[-3:], last @ w4, _mx.product_bound(last, w4, n) + 1e-30, "dx")
+    last = y[:, -3:].cpu().double()
+    _mx.check(dw[-3:], last.t() @ x8, _mx.product_bound(last.t(), x8, m) + 1e-30, "dw")
+    del dx, dw
+    for fmt in ("fp4", "int8"):
+        codes, scales = ops.mx_quantize(y, fmt)
+        tail = ops.mx_quantize(y[-3:].contiguous(), fmt)
+        assert torch.equal(codes[-3:], tail[0])
+        z = ops.mx_dequantize(codes, scales, n, fmt, out_dtype=torch.bfloat16)
+        assert torch.equal(z[-3:], ops.mx_dequantize(*tail, n, fmt, out_dtype=torch.bfloat16))
+        del codes, scales, z
+
+
 # ---- refusals -------------------------------------------------------------------------------------
 
 def test_refusals(cuda_device):
