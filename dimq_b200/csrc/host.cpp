@@ -900,6 +900,26 @@ MxForward mx_layer_forward(const Tensor& x, const Tensor& weight, const OptTenso
   return f;
 }
 
+// Gradients that are made where gradients are recorded (create_graph): whoever differentiates them again is told.
+void differentiable_once(torch::autograd::variable_list& grads, const char* what) {
+  torch::autograd::variable_list parts;
+  for (auto& t : grads)
+    if (t.defined()) parts.push_back(t.detach().requires_grad_(true));
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", static_cast<int64_t>(parts.size()));
+  parts = (*error)(std::move(parts));
+  size_t i = 0;
+  for (auto& t : grads)
+    if (t.defined()) t = parts[i++];
+}
+
+// The result of a gradient entry point: not a constant where grad has a gradient of its own
+Tensor once_of(const Tensor& grad, Tensor result, const char* what) {
+  if (!at::GradMode::is_enabled() || !grad.requires_grad()) return result;
+  torch::autograd::variable_list one = {std::move(result)};
+  differentiable_once(one, what);
+  return one[0];
+}
+
 Tensor mx_grad_scratch(const Tensor& dy, int dyd, int64_t m, int64_t n, int64_t k, int64_t* need) {
   check(dimq_mx_grad_workspace_bytes(dyd, m, n, k, need), "mx_grad_workspace_bytes");
   return scratch(*need, dy);
@@ -943,6 +963,96 @@ Tensor mx_grad_weight(const Tensor& dy, const Tensor& codes, const Tensor& scale
                             nullptr, 0, m, n, k, ws.data_ptr(), need, stream_of(dy)), "mx_linear_grad_weight");
   *launches += m > 0 ? 2 : 0;
   return dw;
+}
+
+// A product whose x, bias or residual has a gradient: straight through x's rounding, dx = dz w^ and dbias the column sums of dz
+// for dz = the gradient in front of the activation.  ReLU's comes from the result; what GELU, and a ReLU whose result has the
+// residual on top, came from is computed again from x.
+class MxProduct : public torch::autograd::Function<MxProduct> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& codes, const Tensor& scales,
+                        const OptTensor& bias, const OptTensor& residual, int64_t n, int64_t k, int64_t out_dtype, int64_t epilogue) {
+    int launches = 0;
+    Tensor y = mx_linear(x, codes, scales, bias, n, k, static_cast<at::ScalarType>(out_dtype), static_cast<int>(epilogue), residual, &launches);
+    count_launches_no_gil(launches);
+    const bool again = epilogue == DIMQ_EPI_GELU || (epilogue == DIMQ_EPI_RELU && residual.has_value());
+    const bool from_y = epilogue == DIMQ_EPI_ADD_RELU || (epilogue == DIMQ_EPI_RELU && !residual.has_value());
+    ctx->save_for_backward({codes, scales, again ? x : Tensor(), again && bias.has_value() ? *bias : Tensor(), from_y ? y : Tensor()});
+    ctx->saved_data["n"] = n;
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["epilogue"] = epilogue;
+    ctx->saved_data["x"] = static_cast<int64_t>(x.scalar_type());
+    if (bias.has_value()) {
+      ctx->saved_data["bias"] = bias->sizes();
+      ctx->saved_data["bias_type"] = static_cast<int64_t>(bias->scalar_type());
+    }
+    if (residual.has_value()) ctx->saved_data["residual"] = residual->sizes();
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(9);
+    if (!grads[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const int64_t n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt(), epilogue = ctx->saved_data["epilogue"].toInt();
+    const bool has_bias = ctx->saved_data.count("bias") != 0, has_residual = ctx->saved_data.count("residual") != 0;
+    // edges are counted over the tensors that were given
+    const bool need_x = ctx->needs_input_grad(0), need_b = has_bias && ctx->needs_input_grad(3);
+    const bool need_r = has_residual && ctx->needs_input_grad(has_bias ? 4 : 3);
+    int launches = 0;
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor dy = grads[0].detach();
+      const c10::cuda::CUDAGuard guard(dy.device());
+      Tensor dz = dy;
+      if (epilogue != DIMQ_EPI_NONE && (need_x || need_b || epilogue == DIMQ_EPI_ADD_RELU)) {
+        if (saved[4].defined()) {
+          dz = at::threshold_backward(dy, saved[4].detach(), 0);
+        } else {
+          const OptTensor bias = saved[3].defined() ? OptTensor(saved[3].detach()) : std::nullopt;
+          const Tensor z = mx_linear(saved[2].detach(), saved[0], saved[1], bias, n, k, at::kFloat, DIMQ_EPI_NONE, std::nullopt, &launches);
+          dz = epilogue == DIMQ_EPI_GELU ? at::gelu_backward(dy.to(at::kFloat), z) : at::threshold_backward(dy.to(at::kFloat), z, 0);
+          dz = dz.to(dy.scalar_type());
+        }
+      }
+      if (need_x || need_b) {
+        int64_t rows = n;
+        Mx w;
+        if (need_x) w = mx_operand(saved[0], saved[1], &rows, k, DIMQ_MX_FP4, "weight");
+        const int dzd = dtype_code(dz, "grad");
+        const Tensor g = aligned16(dz);
+        const int64_t m = mx_rows(g, n);
+        const auto opt = g.options().memory_format(at::MemoryFormat::Contiguous);
+        Tensor dx, db;
+        if (need_x) dx = at::empty(out_shape(g, k), opt.dtype(static_cast<at::ScalarType>(ctx->saved_data["x"].toInt())));
+        if (need_b) db = at::empty(ctx->saved_data["bias"].toIntVector(), opt.dtype(static_cast<at::ScalarType>(ctx->saved_data["bias_type"].toInt())));
+        int64_t need = 0;
+        const Tensor ws = mx_grad_scratch(g, dzd, m, n, k, &need);
+        check(dimq_mx_grads(g.data_ptr(), dzd, need_x ? bytes_of(w.codes) : nullptr, need_x ? bytes_of(w.scales) : nullptr, nullptr, nullptr, 0,
+                            need_x ? dx.data_ptr() : nullptr, need_x ? dtype_code(dx, "gradient") : 0, nullptr, 0,
+                            need_b ? db.data_ptr() : nullptr, need_b ? dtype_code(db, "gradient") : 0, m, n, k, ws.data_ptr(), need,
+                            stream_of(g)), "mx_grads");
+        launches += m > 0 ? 2 * need_x + need_b : 0;
+        out[0] = dx;
+        out[3] = db;
+      }
+      if (need_r) {
+        out[4] = (epilogue == DIMQ_EPI_ADD_RELU ? dz : dy).reshape(ctx->saved_data["residual"].toIntVector());
+      }
+    }
+    count_launches_no_gil(launches);
+    if (at::GradMode::is_enabled()) differentiable_once(out, "mx_linear");
+    return out;
+  }
+};
+
+// The product of the Python entry point: an autograd node where a gradient has to come back.
+Tensor mx_product(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& bias, int64_t n, int64_t k,
+                  at::ScalarType out_dtype, int epilogue, const OptTensor& residual, int* launches) {
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || (bias.has_value() && bias->requires_grad()) || (residual.has_value() && residual->requires_grad())))
+    return MxProduct::apply(x, codes, scales, bias, residual, n, k, static_cast<int64_t>(out_dtype), static_cast<int64_t>(epilogue));
+  return mx_linear(x, codes, scales, bias, n, k, out_dtype, epilogue, residual, launches);
 }
 
 // Gradients straight through the rounding, from what the forward kept.  Differentiable once: a second derivative raises.
@@ -1007,16 +1117,7 @@ class MxLayer : public torch::autograd::Function<MxLayer> {
     out[0] = dx;
     out[1] = dw;
     out[2] = db;
-    if (at::GradMode::is_enabled()) {     // create_graph: whoever differentiates these again is told
-      torch::autograd::variable_list parts;
-      for (auto& t : out)
-        if (t.defined()) parts.push_back(t.detach().requires_grad_(true));
-      auto error = std::make_shared<torch::autograd::DelayedError>("mx_linear is differentiable once", static_cast<int64_t>(parts.size()));
-      parts = (*error)(std::move(parts));
-      size_t i = 0;
-      for (auto& t : out)
-        if (t.defined()) t = parts[i++];
-    }
+    if (at::GradMode::is_enabled()) differentiable_once(out, "mx_linear");
     return out;
   }
 };
@@ -1272,7 +1373,7 @@ PyObject* py_mx_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int epilogue = static_cast<int>(as_int(a[7]));
   int launches = 0;
   Tensor y;
-  { NO_GIL; y = mx_linear(x, codes, scales, bias, out_f, in_f, dt, epilogue, residual, &launches); }
+  { NO_GIL; y = mx_product(x, codes, scales, bias, out_f, in_f, dt, epilogue, residual, &launches); }
   count_launches(launches);
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
@@ -1298,7 +1399,7 @@ PyObject* py_mx_grad_input(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::ScalarType dt = as_dtype(a[4]);
   int launches = 0;
   Tensor dx;
-  { NO_GIL; dx = mx_grad_input(dy, codes, scales, k, dt, &launches); }
+  { NO_GIL; dx = once_of(dy, mx_grad_input(dy, codes, scales, k, dt, &launches), "mx_linear_grad_input"); }
   count_launches(launches);
   return THPVariable_Wrap(dx);
   END_HANDLE_TH_ERRORS
@@ -1313,7 +1414,7 @@ PyObject* py_mx_grad_weight(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::ScalarType dt = as_dtype(a[5]);
   int launches = 0;
   Tensor dw;
-  { NO_GIL; dw = mx_grad_weight(dy, codes, scales, k, format, dt, &launches); }
+  { NO_GIL; dw = once_of(dy, mx_grad_weight(dy, codes, scales, k, format, dt, &launches), "mx_linear_grad_weight"); }
   count_launches(launches);
   return THPVariable_Wrap(dw);
   END_HANDLE_TH_ERRORS

@@ -217,7 +217,8 @@ class MXLinear(nn.Module):
     """Linear layer in microscaled 4-bit numbers: the weight as codes and scales, the activations quantised in the call.
 
     ``from_linear`` takes a float layer (a trained ``nn.Linear`` or one trained with ``qat.mx_linear``, whose forward this
-    repeats); the constructor takes what ``ops.mx_quantize(weight, "fp4")`` returns.
+    repeats); the constructor takes what ``ops.mx_quantize(weight, "fp4")`` returns.  The weight is frozen; gradients of the input
+    and the residual go through.
     """
 
     def __init__(self, weight_codes: torch.Tensor, weight_scales: torch.Tensor, out_features: int, in_features: int,

@@ -651,6 +651,9 @@ def mx_linear(x: torch.Tensor, weight_codes: torch.Tensor, weight_scales: torch.
     ``q(x)`` is ``x`` rounded by ``mx_quantize(x, "fp4")``; ``weight_codes`` / ``weight_scales`` are what
     ``mx_quantize(weight, "fp4")`` returns for the ``[out_features, in_features]`` weight.  Output type, epilogue and
     residual as in :func:`dimq_linear_wq`.
+
+    Gradients of ``x``, ``bias`` and ``residual`` go through (the weight is packed: it has none): straight through the rounding
+    of ``x``, through the activation at the sums in fp32 or the result.  Differentiable once.
     """
     return _lib.host().mx_linear(x, weight_codes, weight_scales, bias, out_features, in_features, out_dtype,
                                  _EPILOGUES[epilogue], residual)
