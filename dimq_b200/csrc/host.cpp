@@ -1070,6 +1070,7 @@ class MxLayer : public torch::autograd::Function<MxLayer> {
     ctx->saved_data["x"] = static_cast<int64_t>(x.scalar_type());
     ctx->saved_data["w"] = static_cast<int64_t>(weight.scalar_type());
     ctx->saved_data["b"] = bias.has_value() ? static_cast<int64_t>(bias->scalar_type()) : int64_t{-1};
+    if (bias.has_value()) ctx->saved_data["b_sizes"] = bias->sizes();   // any shape of n values
     return f.y;
   }
 
@@ -1099,7 +1100,7 @@ class MxLayer : public torch::autograd::Function<MxLayer> {
     Tensor dx, dw, db;
     if (need_x) dx = at::empty(out_shape(g, k), opt.dtype(type("x")));
     if (need_w) dw = at::empty({n, k}, opt.dtype(type("w")));
-    if (need_b) db = at::empty({n}, opt.dtype(type("b")));
+    if (need_b) db = at::empty(ctx->saved_data["b_sizes"].toIntVector(), opt.dtype(type("b")));
     if (!need_x && !need_w && !need_b) return out;
     MxBuffer x, w;
     if (need_w) x = kept(saved[0], g, m, k, keep);
