@@ -339,17 +339,19 @@ mx_add_slices_kernel(const float* __restrict__ partial, int slices, int64_t n, T
   }
 }
 
-// Column sums: a block takes 256 columns of a run of rows, its eight warps the rows in turn; the runs' sums are added by a
-// second kernel, in order.  VEC: rows of whole 16-byte pieces, a lane has eight neighbours; else columns 32 apart.
+// Column sums: a block takes 256 columns of a run of rows (the grid is one dimension: run, then columns), its eight warps the
+// rows in turn; the runs' sums are added by a second kernel, in order.  VEC: rows of whole 16-byte pieces, a lane has eight
+// neighbours; else columns 32 apart.
 constexpr int kSumRows = 256;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-mx_column_sum_kernel(const T* __restrict__ dy, int64_t rows, int64_t cols, float* __restrict__ partial, void* __restrict__ out,
-                     int out_dtype) {
+mx_column_sum_kernel(const T* __restrict__ dy, int64_t rows, int64_t cols, unsigned col_tiles, float* __restrict__ partial,
+                     void* __restrict__ out, int out_dtype) {
   __shared__ float part[8][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 256;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
+  const unsigned run = blockIdx.x / col_tiles;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x - run * col_tiles) * 256;
+  const int64_t r0 = static_cast<int64_t>(run) * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
   float s[8] = {};
 #pragma unroll 4
   for (int64_t r = r0 + warp; r < r1; r += 8) {
@@ -375,7 +377,7 @@ mx_column_sum_kernel(const T* __restrict__ dy, int64_t rows, int64_t cols, float
   if (j >= cols) return;
   float t = part[0][threadIdx.x];
   for (int i = 1; i < 8; ++i) t += part[i][threadIdx.x];
-  if (gridDim.y > 1) partial[blockIdx.y * cols + j] = t;
+  if (rows > kSumRows) partial[run * cols + j] = t;
   else store_from_float(out, out_dtype, j, t);
 }
 __global__ void __launch_bounds__(128)
@@ -391,11 +393,11 @@ mx_column_sum_finish_kernel(const float* __restrict__ partial, int64_t runs, int
 template <typename T>
 int column_sum(const void* dy, int64_t M, int64_t N, float* partial, void* db, int db_dtype, cudaStream_t st) {
   const int64_t runs = (M + kSumRows - 1) / kSumRows, gx = (N + 255) / 256;
-  if (runs > 65535) return DIMQ_ERR_TOO_LARGE;
-  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(runs));
+  if (gx > 0x7FFFFFFF / runs) return DIMQ_ERR_TOO_LARGE;   // 1.4e14 values
+  const unsigned cols = static_cast<unsigned>(gx), grid = cols * static_cast<unsigned>(runs);
   const T* in = static_cast<const T*>(dy);
-  if ((N * static_cast<int64_t>(sizeof(T))) % 16 == 0) mx_column_sum_kernel<T, true><<<grid, 256, 0, st>>>(in, M, N, partial, db, db_dtype);
-  else mx_column_sum_kernel<T, false><<<grid, 256, 0, st>>>(in, M, N, partial, db, db_dtype);
+  if ((N * static_cast<int64_t>(sizeof(T))) % 16 == 0) mx_column_sum_kernel<T, true><<<grid, 256, 0, st>>>(in, M, N, cols, partial, db, db_dtype);
+  else mx_column_sum_kernel<T, false><<<grid, 256, 0, st>>>(in, M, N, cols, partial, db, db_dtype);
   const int rc = launch_status();
   if (rc != DIMQ_OK || runs == 1) return rc;
   mx_column_sum_finish_kernel<<<static_cast<unsigned>((N + 127) / 128), 128, 0, st>>>(partial, runs, N, db, db_dtype);
