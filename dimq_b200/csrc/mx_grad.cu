@@ -11,7 +11,9 @@
 // same reduction, smallest first.
 //
 // The tensor cores cut their sums to fp32 instead of rounding them: the error grows with the number of steps.  Where the
-// result is fp32 it is therefore added up in registers, 512 values of the reduction at a time.
+// result is fp32 it is therefore added up in registers, 512 values of the reduction at a time.  A 16-bit result has room for
+// some of that error: it is added up so where one accumulator would take more than 16384 (fp16) or 131072 (bf16) values of
+// the reduction (long_steps).
 //
 // Tile: 128 rows x BN columns of the result, ring stages of 64 of the reduction, two accumulators in tensor memory.
 // Warps 0-2 fetch, taking the stages in turn, warp 3 issues the MMAs, warps 4-11 are the epilogue, two to a lane quarter.
@@ -100,7 +102,7 @@ __device__ __forceinline__ Unit unit_of(int u, int steps, const GradParams& p) {
   return w;
 }
 
-// SEG: fp32 results of long sums, added up in registers.  PAIR: two blocks share a tile of 256 rows (BN = 256).
+// SEG: long sums, added up in registers.  PAIR: two blocks share a tile of 256 rows (BN = 256).
 template <int BN, int ES, bool SEG, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
@@ -473,6 +475,11 @@ int64_t slices_bytes(int64_t R, int64_t K, int64_t depth, int terms) {
   return s > 1 ? up(R * K * 4 * s, 256) : 0;
 }
 
+// Steps (of 64 values, of one term: the smaller terms' sums are small) after which an accumulator's cuts would count in a
+// 16-bit result.  Values of one sign lose 8e-8 of the sum per 16 values: 6.5e-4 of an fp16 weight gradient over a million
+// rows (in 16 slices), more than half a step of fp16 (4.9e-4).  These limits keep that below a sixth of half a step.
+int64_t long_steps(int dtype) { return dtype == DIMQ_F16 ? 256 : 2048; }
+
 // out [R][K] = A * decoded, A = dy (reduction over its columns) or dy^T (over its rows, a_cols); `depth` values reduced
 int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms, bool a_cols, const void* decoded, int64_t depth, int64_t K,
                  Out out, void* partial, cudaStream_t st) {
@@ -511,13 +518,17 @@ int grad_product(const void* dy, int64_t M, int64_t N, int64_t pitch, int terms,
       !encode_map(&maps.b, bf16, 3, decoded, bdims, bstr, bbox, CU_TENSOR_MAP_SWIZZLE_128B) ||
       (out.tma && !encode_out(&maps.y, rows_of_all)))
     return DIMQ_ERR_DRIVER;
-  const bool wide = result.dtype == DIMQ_F32, seg = wide && p.depth_blocks * terms > kSegStages * plan.slices;
+  const bool wide = result.dtype == DIMQ_F32;
+  const int64_t steps = static_cast<int64_t>(p.depth_blocks) * terms, share = (steps + plan.slices - 1) / plan.slices;
+  const bool seg = wide ? steps > kSegStages * plan.slices
+                        : (share < p.depth_blocks ? share : p.depth_blocks) > long_steps(result.dtype);
   int rc;
 #define DIMQ_MX_GRAD(ES, SEG)                                          \
   rc = pair ? launch_grad<256, ES, SEG, true>(maps, p, st)             \
        : bn == 256 ? launch_grad<256, ES, SEG, false>(maps, p, st)     \
        : bn == 128 ? launch_grad<128, ES, SEG, false>(maps, p, st) : launch_grad<64, ES, SEG, false>(maps, p, st)
-  if (seg) { DIMQ_MX_GRAD(4, true); }
+  if (seg && out.dtype == DIMQ_F32) { DIMQ_MX_GRAD(4, true); }
+  else if (seg) { DIMQ_MX_GRAD(2, true); }
   else if (out.dtype == DIMQ_F32) { DIMQ_MX_GRAD(4, false); }
   else { DIMQ_MX_GRAD(2, false); }
 #undef DIMQ_MX_GRAD

@@ -49,3 +49,24 @@ def test_more_rows_than_a_grid_dimension_has_runs(cuda_device):
     assert torch.equal(dw, (dy.double().t() @ x8.double()).float())
     w4 = ops.mx_dequantize(*ops.mx_quantize(w.detach()), k)
     assert torch.equal(dx[-300:], (dy[-300:].float() @ w4).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype,m,n,k", [(torch.float16, 1 << 20, 64, 64), (torch.float16, 20000, 18944, 64), (torch.float16, 20000, 2432, 832),
+                                         (torch.float16, 20000, 1920, 1216), (torch.float16, 20000, 1152, 3648),
+                                         (torch.bfloat16, 1 << 22, 64, 64), (torch.bfloat16, 140000, 1920, 1216)])
+def test_sums_over_many_rows_in_16_bits(cuda_device, m, n, k, dtype):
+    """Weight gradients whose terms have one sign, over up to four million rows (in slices, and whole with every tile width):
+    half a step of their 16-bit type from 64 bits and little more.
+
+    Little: sums of 512 values take 32 steps of the tensor cores, each off by at most two units of 2^-23 of the sum (7.6e-6),
+    and at most 512 + 16 of them are added in fp32 (3.2e-5 of bf16's 3.9e-3; at most 272 for fp16, 1.6e-5 of 4.9e-4)."""
+    from dimq_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    dy = ((torch.rand(m, n, device="cuda", generator=gen) + 0.5) / 1024).to(dtype)
+    kept = ops.mx_quantize((torch.rand(m, k, device="cuda", generator=gen) + 0.5).to(torch.bfloat16), "int8")
+    g = ops.mx_linear_grad_weight(dy, *kept, k, "int8", out_dtype=dtype).double()
+    x8 = ops.mx_dequantize(*kept, k, "int8")
+    want = sum(dy[r:r + 65536].double().t() @ x8[r:r + 65536].double() for r in range(0, m, 65536))
+    worst = float(((g - want).abs() / want).max())
+    assert worst <= torch.finfo(dtype).eps / 2 + 64 * 2.0 ** -23 + (288 if dtype == torch.float16 else 528) * 2.0 ** -24, worst
