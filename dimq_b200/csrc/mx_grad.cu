@@ -263,7 +263,7 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
           __syncwarp();
           if constexpr (!SEG) {
             const int64_t n0 = n_first + (sub + 2 * i) * 32;
-            if (row0 < out.rows && n0 < out.cols) put_chunk<ES>(sum[0], out, &maps.y, stage, piece, nullptr, row0, n0, lane);
+            if (row0 < out.rows && n0 < out.cols) put_chunk<ES, false>(sum[0], out, &maps.y, stage, piece, nullptr, row0, n0, lane);
           }
         }
         if (++buf == 2) { buf = 0; bph ^= 1u; }
@@ -273,7 +273,7 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
           const int64_t n0 = n_first + (sub + 2 * i) * 32;
-          if (row0 < out.rows && n0 < out.cols) put_chunk<ES>(sum[i], out, &maps.y, stage, piece, nullptr, row0, n0, lane);
+          if (row0 < out.rows && n0 < out.cols) put_chunk<ES, false>(sum[i], out, &maps.y, stage, piece, nullptr, row0, n0, lane);
         }
       }
     }

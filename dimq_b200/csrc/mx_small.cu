@@ -222,7 +222,8 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
     if (p.out.bias != nullptr) s += load_as_float(p.out.bias, p.out.bias_dtype, n);
     const int64_t o = m * p.out.cols + n;
     const float res = p.out.residual != nullptr ? load_as_float(p.out.residual, p.out.dtype, o) : 0.0f;
-    store_from_float(p.out.y, p.out.dtype, o, activate_any(s, res, p.out.epilogue));
+    store_from_float(p.out.y, p.out.dtype, o,
+                     p.out.dtype == DIMQ_F32 ? activate_any<true>(s, res, p.out.epilogue) : activate_any<false>(s, res, p.out.epilogue));
   }
   __syncwarp();
   if (slices > 1) {         // no block leaves while a peer may read its sums

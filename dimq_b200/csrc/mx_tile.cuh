@@ -174,18 +174,21 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN stays on
   return d;
 }
 
-template <int EPI>
-__device__ __forceinline__ float activate(float v, float res) {
-  if (EPI == DIMQ_EPI_ADD_RELU) return max_nan(v + res, 0.0f);
-  if (EPI == DIMQ_EPI_RELU) v = max_nan(v, 0.0f);
-  if (EPI == DIMQ_EPI_GELU) v = 0.5f * v * (1.0f + fast_erf(v * 0.70710678118654752440f));
+// GELU of a result in 16 bits takes the polynomial error function (1.5e-7 of v, in the tail most of GELU: at v = -5, 4 %); of
+// one in fp32 the complementary error function, good to a few steps in relative terms wherever GELU is a normal number.
+__device__ __forceinline__ float gelu_fast(float v) { return 0.5f * v * (1.0f + fast_erf(v * 0.70710678118654752440f)); }
+__device__ __forceinline__ float gelu_wide(float v) { return 0.5f * v * erfcf(v * -0.70710678118654752440f); }
+
+// RELU, ADD_RELU or none
+__device__ __forceinline__ float activate_linear(float v, float res, int epilogue) {
+  if (epilogue == DIMQ_EPI_ADD_RELU) return max_nan(v + res, 0.0f);
+  if (epilogue == DIMQ_EPI_RELU) v = max_nan(v, 0.0f);
   return v + res;
 }
+template <bool WIDE>
 __device__ __forceinline__ float activate_any(float v, float res, int epilogue) {
-  if (epilogue == DIMQ_EPI_NONE) return v + res;
-  if (epilogue == DIMQ_EPI_RELU) return activate<DIMQ_EPI_RELU>(v, res);
-  if (epilogue == DIMQ_EPI_GELU) return activate<DIMQ_EPI_GELU>(v, res);
-  return activate<DIMQ_EPI_ADD_RELU>(v, res);
+  if (epilogue == DIMQ_EPI_GELU) return (WIDE ? gelu_wide(v) : gelu_fast(v)) + res;
+  return activate_linear(v, res, epilogue);
 }
 
 struct Out {            // where a product goes
@@ -215,7 +218,9 @@ constexpr uint32_t kStagingBytes = 4096;
 // sums change hands through shared memory, so that a warp stores 32 neighbours of one row at a time.  (Boxes of 64 columns,
 // and 16-byte stores of four rows at a time instead of the map, were slower: 25216 x 768 -> 2304 bf16 59 and 69 us against
 // 57.)
-template <int ES>
+// GELU of fp32 is done in the box, four values at a time: unrolled over the row in registers it would not fit.  (ACT: whether
+// there can be an activation.)
+template <int ES, bool ACT = true>
 __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CUtensorMap* map, unsigned char* stage, uint32_t& turn,
                                           const float* bias, int64_t row0, int64_t n0, int lane) {
   if (o.tma) {
@@ -227,7 +232,8 @@ __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CU
         v[4 * j] += b.x; v[4 * j + 1] += b.y; v[4 * j + 2] += b.z; v[4 * j + 3] += b.w;
       }
     }
-    if (o.residual != nullptr) {
+    const bool in_box = ES == 4 && ACT && o.epilogue == DIMQ_EPI_GELU;
+    if (o.residual != nullptr && !in_box) {
       constexpr int kPer = 16 / ES;
       const char* r = static_cast<const char*>(o.residual) + (row * o.cols + n0) * ES;
 #pragma unroll
@@ -235,11 +241,16 @@ __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CU
         uint4 q = make_uint4(0u, 0u, 0u, 0u);
         if (row < o.rows && n0 + c * kPer < o.cols) q = __ldg(reinterpret_cast<const uint4*>(r) + c);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) v[c * kPer + i] = activate_any(v[c * kPer + i], element<ES>(q, i, o.dtype), o.epilogue);
+        for (int i = 0; i < kPer; ++i) {
+          const float res = element<ES>(q, i, o.dtype);
+          v[c * kPer + i] = ES == 2 ? activate_any<false>(v[c * kPer + i], res, o.epilogue) : activate_linear(v[c * kPer + i], res, o.epilogue);
+        }
       }
     } else if (o.epilogue == DIMQ_EPI_GELU) {
+      if (ES == 2) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = activate<DIMQ_EPI_GELU>(v[j], 0.0f);
+        for (int j = 0; j < 32; ++j) v[j] = gelu_fast(v[j]);
+      }
     } else if (o.epilogue != DIMQ_EPI_NONE) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = max_nan(v[j], 0.0f);
@@ -271,6 +282,17 @@ __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CU
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         *reinterpret_cast<float4*>(p + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      if (in_box) {
+        const float* r = static_cast<const float*>(o.residual) + row * o.cols + n0;
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {   // the lane's own row
+          float4* at = reinterpret_cast<float4*>(p + ((j ^ (lane & 7)) << 4));
+          float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f), g = *at;
+          if (o.residual != nullptr && row < o.rows && n0 + 4 * j < o.cols) q = __ldg(reinterpret_cast<const float4*>(r) + j);
+          g.x = gelu_wide(g.x) + q.x; g.y = gelu_wide(g.y) + q.y; g.z = gelu_wide(g.z) + q.z; g.w = gelu_wide(g.w) + q.w;
+          *at = g;
+        }
+      }
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -295,7 +317,7 @@ __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CU
     for (int r = 0; r < rows; ++r) {
       const int64_t at = (row0 + r) * o.cols + n;
       const float res = o.residual != nullptr ? load_as_float(o.residual, o.dtype, at) : 0.0f;
-      store_from_float(o.y, o.dtype, at, activate_any(f[r * 32 + (lane ^ r)] + b, res, o.epilogue));
+      store_from_float(o.y, o.dtype, at, ACT ? activate_any<ES == 4>(f[r * 32 + (lane ^ r)] + b, res, o.epilogue) : f[r * 32 + (lane ^ r)] + b);
     }
   }
   __syncwarp();

@@ -372,8 +372,9 @@ DIMQ_API int dimq_mx_dequantize(const void* codes, const uint8_t* scales, int fo
                                 int out_dtype, void* stream);
 
 /* y [M][N] = epilogue(x^ w^T + bias) + residual, x^ the DIMQ_MX_FP4 values of x [M][K], w^ those of w_codes / w_scales
- * ([N][K]), products and sums in fp32.  Bias, epilogue and residual as in dimq_linear_wq (residual: y's type).  With
- * x_scales != NULL, x holds the codes of x^ already (x_dtype is not looked at).  Scratch:
+ * ([N][K]), products and sums in fp32.  Bias, epilogue and residual as in dimq_linear_wq (residual: y's type), but that
+ * a NaN passes the ReLUs and that GELU of an fp32 y keeps its digits in the tail (erfc; 16-bit types: a polynomial, 1.5e-7 of
+ * the argument).  With x_scales != NULL, x holds the codes of x^ already (x_dtype is not looked at).  Scratch:
  * dimq_mx_linear_workspace_bytes (coded: whether x_scales is given), 16-byte aligned. */
 DIMQ_API int dimq_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int coded, int64_t* bytes);
 DIMQ_API int dimq_mx_linear(const void* x, int x_dtype, const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales,
