@@ -880,23 +880,33 @@ MxForward mx_layer_forward(const Tensor& x, const Tensor& weight, const OptTenso
   void* st = stream_of(x);
   const Tensor xc = x.contiguous(), wc = weight.contiguous();
   const int64_t m = mx_rows(x, k);
-  const MxBuffer w4 = mx_buffer(n, k, DIMQ_MX_FP4, x), x4 = mx_buffer(m, k, DIMQ_MX_FP4, x);
+  const MxBuffer w4 = mx_buffer(n, k, DIMQ_MX_FP4, x);
   MxForward f;
   check(dimq_mx_quantize(wc.data_ptr(), wd, n, k, DIMQ_MX_FP4, w4.codes(), w4.scales(), st), "mx_quantize");
+  // A few rows are quantised by the product itself: the kernel that mx_linear runs for them, so that a layer deployed from
+  // this one gives its bits.
+  int64_t room = 0;
+  check(dimq_mx_linear_workspace_bytes(m, n, k, 0, &room), "mx_linear_workspace_bytes");
+  const bool few = m > 0 && room == 0;
+  MxBuffer x4;
+  if (!few || keep == DIMQ_MX_FP4) x4 = mx_buffer(m, k, DIMQ_MX_FP4, x);
   if (keep == DIMQ_MX_INT8) {
     const MxBuffer x8 = mx_buffer(m, k, DIMQ_MX_INT8, x);
-    check(dimq_mx_quantize_both(xc.data_ptr(), xd, m, k, x4.codes(), x4.scales(), reinterpret_cast<int8_t*>(x8.codes()), x8.scales(), st),
-          "mx_quantize_both");
+    if (few)
+      check(dimq_mx_quantize(xc.data_ptr(), xd, m, k, DIMQ_MX_INT8, x8.codes(), x8.scales(), st), "mx_quantize");
+    else
+      check(dimq_mx_quantize_both(xc.data_ptr(), xd, m, k, x4.codes(), x4.scales(), reinterpret_cast<int8_t*>(x8.codes()), x8.scales(), st),
+            "mx_quantize_both");
     f.x = x8.t;
-  } else {
+  } else if (!few || keep == DIMQ_MX_FP4) {
     check(dimq_mx_quantize(xc.data_ptr(), xd, m, k, DIMQ_MX_FP4, x4.codes(), x4.scales(), st), "mx_quantize");
     if (keep == DIMQ_MX_FP4) f.x = x4.t;
   }
   if (keep_w) f.w = w4.t;
   f.y = at::empty(out_shape(x, n), x.options().memory_format(at::MemoryFormat::Contiguous));
-  check(dimq_mx_linear(x4.codes(), 0, x4.scales(), w4.codes(), w4.scales(), ptr(b.t), b.dtype, nullptr, f.y.data_ptr(),
-                       dtype_code(f.y, "y"), m, n, k, DIMQ_EPI_NONE, nullptr, 0, st), "mx_linear");
-  *launches += 1 + 2 * (m > 0);
+  check(dimq_mx_linear(few ? xc.data_ptr() : x4.codes(), xd, few ? nullptr : x4.scales(), w4.codes(), w4.scales(), ptr(b.t), b.dtype, nullptr,
+                       f.y.data_ptr(), dtype_code(f.y, "y"), m, n, k, DIMQ_EPI_NONE, nullptr, 0, st), "mx_linear");
+  *launches += 1 + (m > 0) + (m > 0 && (!few || keep != 0));
   return f;
 }
 

@@ -70,3 +70,32 @@ def test_sums_over_many_rows_in_16_bits(cuda_device, m, n, k, dtype):
     want = sum(dy[r:r + 65536].double().t() @ x8[r:r + 65536].double() for r in range(0, m, 65536))
     worst = float(((g - want).abs() / want).max())
     assert worst <= torch.finfo(dtype).eps / 2 + 64 * 2.0 ** -23 + (288 if dtype == torch.float16 else 528) * 2.0 ** -24, worst
+
+
+def _spread(rows, cols, seed):
+    """Normal values whose blocks of 32 differ by up to 2^24: sums that fp32 has to round."""
+    gen = torch.Generator().manual_seed(seed)
+    e = torch.randint(-12, 13, (rows, (cols + 31) // 32), generator=gen).float().repeat_interleave(32, 1)[:, :cols]
+    return (torch.randn(rows, cols, generator=gen) * torch.exp2(e)).cuda()
+
+
+@pytest.mark.parametrize("checkpoint", ["int8", "fp4", None])
+@pytest.mark.parametrize("m,k,n", [(1, 8192, 72), (4, 4100, 40), (16, 8192, 130), (17, 1000, 64), (32, 8192, 72), (40, 8192, 72), (200, 1030, 300)])
+def test_trained_and_deployed_products_have_the_same_bits(cuda_device, m, k, n, checkpoint):
+    """Whatever the number of rows, and where the order of a sum shows (None: nothing needs a gradient)."""
+    from dimq_b200 import ops, qat
+
+    x, w = _spread(m, k, 4), _spread(n, k, 5)
+    b = torch.randn(n, device="cuda")
+    want = ops.mx_linear(x, *ops.mx_quantize(w), b, n, k)
+    if checkpoint is None:
+        assert torch.equal(qat.mx_linear(x, w, b), want)
+        return
+    x.requires_grad_(), w.requires_grad_()
+    y = qat.mx_linear(x, w, b, checkpoint=checkpoint)
+    assert torch.equal(y, want)
+    dy = _spread(m, n, 6)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)          # what is kept is what the operators quantise
+    kept = ops.mx_quantize(x.detach(), checkpoint)
+    assert torch.equal(dw, ops.mx_linear_grad_weight(dy, *kept, k, checkpoint))
+    assert torch.equal(dx, ops.mx_linear_grad_input(dy, *ops.mx_quantize(w.detach()), k))
