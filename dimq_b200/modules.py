@@ -217,8 +217,8 @@ class MXLinear(nn.Module):
     """Linear layer in microscaled 4-bit numbers: the weight as codes and scales, the activations quantised in the call.
 
     ``from_linear`` takes a float layer (a trained ``nn.Linear`` or one trained with ``qat.mx_linear``, whose forward this
-    repeats); the constructor takes what ``ops.mx_quantize(weight, "fp4")`` returns.  The weight is frozen; gradients of the input
-    and the residual go through.
+    repeats bit for bit); the constructor takes what ``ops.mx_quantize(weight, "fp4")`` returns.  The result has the input's type
+    unless ``out_dtype`` names another.  The weight is frozen; gradients of the input and the residual go through.
     """
 
     def __init__(self, weight_codes: torch.Tensor, weight_scales: torch.Tensor, out_features: int, in_features: int,
@@ -241,7 +241,7 @@ class MXLinear(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         return ops.mx_linear(x, self.weight_codes, self.weight_scales, self.bias, self.out_features, self.in_features,
-                             out_dtype=self.out_dtype, epilogue=self.epilogue, residual=residual)
+                             out_dtype=self.out_dtype or x.dtype, epilogue=self.epilogue, residual=residual)
 
     def extra_repr(self) -> str:
         return f"{self.in_features} -> {self.out_features}, fp4 in blocks of 32"

@@ -99,3 +99,24 @@ def test_trained_and_deployed_products_have_the_same_bits(cuda_device, m, k, n, 
     kept = ops.mx_quantize(x.detach(), checkpoint)
     assert torch.equal(dw, ops.mx_linear_grad_weight(dy, *kept, k, checkpoint))
     assert torch.equal(dx, ops.mx_linear_grad_input(dy, *ops.mx_quantize(w.detach()), k))
+
+
+@pytest.mark.parametrize("m", [1, 20, 150])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_deployed_chain_repeats_the_training_forward(cuda_device, dtype, m):
+    """Two layers: the same types and bits, so that the second one quantises the values it was trained on."""
+    from dimq_b200 import qat
+    from dimq_b200.modules import MXLinear
+
+    torch.manual_seed(0)
+    l1, l2 = torch.nn.Linear(1000, 130).cuda(), torch.nn.Linear(130, 40).cuda()
+    with torch.no_grad():
+        l1.weight.copy_(_spread(130, 1000, 7) * 0.01)
+        x = torch.randn(m, 1000, device="cuda").to(dtype)
+        h = qat.mx_linear(x, l1.weight, l1.bias)
+        want = qat.mx_linear(torch.relu(h), l2.weight, l2.bias)
+    d1, d2 = MXLinear.from_linear(l1, epilogue="relu"), MXLinear.from_linear(l2)
+    got = d1(x)
+    assert got.dtype == h.dtype == dtype and torch.equal(got, torch.relu(h))
+    assert d2(got).dtype == dtype and torch.equal(d2(got), want)
+    assert MXLinear.from_linear(l2, out_dtype=torch.float32)(got).dtype == torch.float32
