@@ -52,6 +52,7 @@ struct GemmHeader {
   uint64_t full[kMaxStages], empty[kMaxStages], d_full[2], d_empty[2];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
+  uint32_t filled[kMaxStages];                   // how often each stage was
 };
 
 template <int BN, bool PAIR>
@@ -82,7 +83,7 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
   const int tile_step = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
+    for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); hdr->filled[s] = 0u; }
     for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), PAIR ? 2 : 1); }
     hdr->abort_flag = 0u;
     fence_barrier_init();
@@ -106,17 +107,18 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
     // no more producers than stages: a warp's successive stages are at most one revolution apart, or the one bit of a
     // barrier's phase could not tell the round it waits for from the one before
     const uint32_t turns = n_st < kProducers ? n_st : kProducers;
-    uint32_t stage = 0, phase = 0, turn = 0, issued = 0;
+    uint32_t stage = 0, round = 0, turn = 0;
     bool ok = true;
     for (int t = tile0; t < p.tiles && ok; t += tile_step) {
       const int n_blk = t % p.n_tiles, m_blk = (PAIR ? 2 : 1) * (t / p.n_tiles) + rank;
       for (int kb = 0; kb < k_stages; ++kb) {
         if (turn == static_cast<uint32_t>(warp)) {
-          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase ^ 1u, abort_flag, 0x2100u | stage))) { ok = false; break; }
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), (round & 1u) ^ 1u, abort_flag, 0x2100u | stage))) { ok = false; break; }
           const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * S::kStageBytes);
           const uint32_t sf = dst + kABytes + S::kBBytes;
           if constexpr (PAIR) {
             if (elect_one()) {     // both blocks' bytes are counted in the first one's barrier
+              hdr->filled[stage] = round + 1u;
               if (rank == 0) mbar_arrive_expect_tx(full, 2 * S::kStageBytes);
               const uint32_t lead = map_to_cta(full, 0);
               tma_load_2d_pair(dst, &maps.a, lead, kb * 128, m_blk * 128);
@@ -129,6 +131,7 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
             const int rt0 = n_blk * BN / 128;
             const int rts = S::kRowTiles < p.row_tiles_b - rt0 ? S::kRowTiles : p.row_tiles_b - rt0;
             if (elect_one()) {
+              hdr->filled[stage] = round + 1u;
               mbar_arrive_expect_tx(full, kABytes + S::kBBytes + sf_bytes * (1 + rts));
               tma_load_2d(dst, &maps.a, full, kb * 128, m_blk * 128);
               tma_load_2d(dst + kABytes, &maps.b, full, kb * 128, n_blk * BN);
@@ -139,18 +142,8 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
           }
           __syncwarp();
         }
-        ++issued;
         if (++turn == turns) turn = 0;
-        if (++stage == n_st) { stage = 0; phase ^= 1u; }
-      }
-    }
-    if (!ok && lane == 0) {   // gave up: bounded wait for the copies in flight, so that none lands after the block has gone
-      const uint32_t n_back = issued < n_st ? issued : n_st;
-      uint32_t s = stage, ph = phase;
-      for (uint32_t i = 0; i < n_back; ++i) {
-        if (s == 0) { s = n_st - 1; ph ^= 1u; } else { --s; }
-        for (uint32_t it = 0; it < kSpinLimit; ++it)
-          if (mbar_try_wait(smem_u32(&hdr->full[s]), ph)) break;
+        if (++stage == n_st) { stage = 0; ++round; }
       }
     }
     __syncwarp();
@@ -248,8 +241,7 @@ mx_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
   }
 
   tc_fence_before();
-  __syncthreads();
-  if constexpr (PAIR) { cluster_arrive(); cluster_wait(); }   // neither block leaves while the other may use its memories
+  leave_together<PAIR>(abort_flag, hdr->full, hdr->filled, n_st, rank);
   if (warp == kProducers) {
     tc_fence_after();
     if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);

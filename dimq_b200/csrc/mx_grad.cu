@@ -50,6 +50,7 @@ struct GradHeader {
   uint64_t full[kMaxStages], empty[kMaxStages], d_full[2], d_empty[2];
   uint32_t tmem_base, drained[2];
   volatile uint32_t abort_flag;
+  uint32_t filled[kMaxStages];                   // how often each stage was
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1, int c2) {
@@ -120,7 +121,7 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
   const int unit_step = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); }
+    for (int s = 0; s < kMaxStages; ++s) { mbar_init(smem_u32(&hdr->full[s]), 1); mbar_init(smem_u32(&hdr->empty[s]), 1); hdr->filled[s] = 0u; }
     for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&hdr->d_full[s]), 1); mbar_init(smem_u32(&hdr->d_empty[s]), PAIR ? 2 : 1); }
     hdr->abort_flag = 0u;
     hdr->drained[0] = hdr->drained[1] = 0u;
@@ -144,7 +145,7 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
   if (warp < kProducers) {
     // no more producers than stages, as in the forward product
     const uint32_t turns = n_st < kProducers ? n_st : kProducers;
-    uint32_t stage = 0, phase = 0, turn = 0, issued = 0;
+    uint32_t stage = 0, round = 0, turn = 0;
     bool ok = true;
     for (int u = unit0; u < units && ok; u += unit_step) {
       const Unit w = unit_of(u, all_steps, p);
@@ -152,9 +153,10 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
       int term = p.terms - 1 - w.first / p.depth_blocks, kb = w.first % p.depth_blocks;   // smallest terms first
       for (int s = w.first; s < w.end; ++s) {
         if (turn == static_cast<uint32_t>(warp)) {
-          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase ^ 1u, abort_flag, 0x3100u | stage))) { ok = false; break; }
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), (round & 1u) ^ 1u, abort_flag, 0x3100u | stage))) { ok = false; break; }
           const uint32_t full = smem_u32(&hdr->full[stage]), dst = smem_u32(smem + stage * kStageBytes);
           if (elect_one()) {     // a pair counts both blocks' bytes in the first one's barrier
+            hdr->filled[stage] = round + 1u;
             if (rank == 0) mbar_arrive_expect_tx(full, (PAIR ? 2 : 1) * kStageBytes);
             const uint32_t bar = PAIR ? map_to_cta(full, 0) : full;
             if (p.a_cols) {
@@ -167,19 +169,9 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
           }
           __syncwarp();
         }
-        ++issued;
         if (++turn == turns) turn = 0;
-        if (++stage == n_st) { stage = 0; phase ^= 1u; }
+        if (++stage == n_st) { stage = 0; ++round; }
         if (++kb == p.depth_blocks) { kb = 0; --term; }
-      }
-    }
-    if (!ok && lane == 0) {   // gave up: bounded wait for the copies in flight
-      const uint32_t n_back = issued < n_st ? issued : n_st;
-      uint32_t s = stage, ph = phase;
-      for (uint32_t i = 0; i < n_back; ++i) {
-        if (s == 0) { s = n_st - 1; ph ^= 1u; } else { --s; }
-        for (uint32_t it = 0; it < kSpinLimit; ++it)
-          if (mbar_try_wait(smem_u32(&hdr->full[s]), ph)) break;
       }
     }
     __syncwarp();
@@ -283,8 +275,7 @@ mx_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
   }
 
   tc_fence_before();
-  __syncthreads();
-  if constexpr (PAIR) { cluster_arrive(); cluster_wait(); }   // neither block leaves while the other may use its memories
+  leave_together<PAIR>(abort_flag, hdr->full, hdr->filled, n_st, rank);
   if (warp == kProducers) {
     tc_fence_after();
     if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);

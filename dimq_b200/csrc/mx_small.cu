@@ -133,6 +133,7 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
   let_dependents_start();       // every block of this grid runs by now and has its columns
   const uint32_t tmem = hdr->tmem_base;
   bool ok = true;
+  int fetched = n_steps < p.stages ? n_steps : p.stages;   // warp 1: steps whose copies have been issued
   if (warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
@@ -161,19 +162,12 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
   } else if (warp == 1) {       // the ring's later rounds
     int stage = 0;
     uint32_t phase = 0;
-    int i = p.stages;
-    for (; i < n_steps; ++i) {
+    for (; fetched < n_steps; ++fetched) {
       if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&hdr->empty[stage]), phase, &hdr->abort_flag, 0x4300u | stage))) { ok = false; break; }
-      if (elect_one()) load_step(i, stage);
+      if (elect_one()) load_step(fetched, stage);
       __syncwarp();
       if (++stage == p.stages) { stage = 0; phase ^= 1u; }
     }
-    if (!ok) {                  // gave up: bounded wait for the copies in flight, the last of every stage
-      for (int j = i - p.stages < 0 ? 0 : i - p.stages; j < i; ++j)
-        for (uint32_t it = 0; it < kSpinLimit; ++it)
-          if (mbar_try_wait(smem_u32(&hdr->full[j % p.stages]), static_cast<uint32_t>(j / p.stages) & 1u)) break;
-    }
-    __syncwarp();
   }
   if (warp < 4) {
     ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(smem_u32(&hdr->done), 0u, &hdr->abort_flag, 0x4200u));
@@ -197,6 +191,11 @@ mx_small_kernel(const __grid_constant__ CUtensorMap codes, const SmallParams p) 
     cluster_wait();
   } else {
     __syncthreads();
+  }
+  if (warp == 1 && hdr->abort_flag != 0u) {   // someone gave up: a bounded wait for the last copies of every stage
+    uint32_t left = kSpinLimit;
+    for (int j = fetched - p.stages < 0 ? 0 : fetched - p.stages; j < fetched; ++j)
+      while (left != 0u && !mbar_try_wait(smem_u32(&hdr->full[j % p.stages]), static_cast<uint32_t>(j / p.stages) & 1u)) --left;
   }
   // each block finishes a share of the weight rows
   const int share = 128 / slices;

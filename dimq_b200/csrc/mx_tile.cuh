@@ -146,6 +146,45 @@ __device__ __forceinline__ void commit(uint32_t bar) {   // PAIR: one arrival in
     mma_commit(bar);
 }
 
+// A block that gave up a wait must not leave while copies into its shared memory are under way.  Its producers note how often
+// they filled each stage; when all warps have stopped, one thread waits (together no longer than one more limit) for the last
+// filling of each.  PAIR: the first block's barriers count both blocks' copies, so it waits for both; a filling that only one
+// of the two began never completes and is waited for as long as the limit allows.
+__device__ __forceinline__ uint32_t peer_word(const uint32_t* at, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(map_to_cta(smem_u32(at), rank)) : "memory");
+  return v;
+}
+template <bool PAIR>
+__device__ __forceinline__ void wait_for_copies(const uint64_t* full, const uint32_t* filled, uint32_t stages) {
+  uint32_t left = kSpinLimit;
+  for (uint32_t s = 0; s < stages; ++s) {
+    uint32_t n = filled[s];
+    if (PAIR) n = max(n, peer_word(filled + s, 1));
+    while (n != 0u && left != 0u && !mbar_try_wait(smem_u32(full + s), (n - 1u) & 1u)) --left;
+  }
+}
+// The end of a block of the persistent kernels, all threads: whether anyone gave up (PAIR: in either block) decides alike for
+// all, and no block of a pair leaves while the other may use its memories.
+template <bool PAIR>
+__device__ __forceinline__ void leave_together(volatile uint32_t* abort_flag, const uint64_t* full, const uint32_t* filled, uint32_t stages,
+                                               int rank) {
+  __syncthreads();
+  if constexpr (PAIR) {
+    if (threadIdx.x == 0 && *abort_flag != 0u)
+      asm volatile("st.shared::cluster.u32 [%0], %1;"
+                   ::"r"(map_to_cta(smem_u32(const_cast<const uint32_t*>(abort_flag)), static_cast<uint32_t>(rank ^ 1))), "r"(1u) : "memory");
+    __syncwarp();             // the cluster's barrier wants whole warps
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (*abort_flag == 0u) return;
+  if (threadIdx.x == 0 && rank == 0) wait_for_copies<PAIR>(full, filled, stages);
+  __syncwarp();
+  if constexpr (PAIR) { cluster_arrive(); cluster_wait(); }
+  else __syncthreads();
+}
+
 // One lane of an epilogue warp whose sums are in registers: the last of the warps hands the accumulator back (PAIR: to the
 // first block's barrier).  Nothing waits here: with two accumulators the warps need not keep step (a barrier among them held
 // the fp32 8192 x 11008 -> 4096 weight gradient at 630 us, 540 so).
