@@ -2,10 +2,12 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
-from tests import _mx
+from tests import _mx, _mx_forms
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +32,95 @@ def test_gelu_of_fp32_results(cuda_device, m, n):
     y = ops.mx_linear(x, *q, v.cuda(), n, 32, epilogue="gelu", residual=r)
     want = want + r.cpu().double()
     _mx.check(y, want, bound + 2.0 ** -24 * (want.abs() + bound))
+
+
+# ---- sums that are exact: every form has to give them to the bit -----------------------------------
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _grid(rows, cols, gen):
+    """4-bit values as they are: signed grid values under block exponents -1, 0 and 1 (multiples of 1/4 up to 12)."""
+    blocks = (cols + 31) // 32
+    v = _mx.GRID.float().cuda()[torch.randint(0, 8, (rows, blocks, 32), device="cuda", generator=gen)]
+    v[:, :, 0] = 4.0 + 2.0 * torch.randint(0, 2, (rows, blocks), device="cuda", generator=gen)     # the block's exponent
+    v = torch.where(torch.rand(rows, blocks, 32, device="cuda", generator=gen) < 0.5, -v, v)
+    e = torch.randint(-1, 2, (rows, blocks, 1), device="cuda", generator=gen).float()
+    return (v * torch.exp2(e)).reshape(rows, -1)[:, :cols].contiguous()
+
+
+def _bytes(rows, cols, gen):
+    """8-bit values as they are: integers up to 127 over 64, one of 64 or more in every block, exponents -1, 0 and 1."""
+    blocks = (cols + 31) // 32
+    c = torch.randint(-127, 128, (rows, blocks, 32), device="cuda", generator=gen).float()
+    c[:, :, 0] = torch.randint(64, 128, (rows, blocks), device="cuda", generator=gen).float()
+    e = torch.randint(-1, 2, (rows, blocks, 1), device="cuda", generator=gen).float()
+    return (c / 64 * torch.exp2(e)).reshape(rows, -1)[:, :cols].contiguous()
+
+
+def _assert_exact(y, a, b, unit, what):
+    """y = a @ b to the bit: products are multiples of `unit` and no partial sum, in whatever order, needs more than 24 bits."""
+    a, b = a.double(), b.double()
+    assert float((a.abs() @ b.abs()).max()) < 2.0 ** 24 * unit, "the data of this test"
+    assert torch.equal(y, (a @ b).to(y.dtype)), what
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("m,k,n", _mx_forms.PRODUCTS)
+def test_products_of_every_form_are_exact(cuda_device, m, k, n, name):
+    from dimq_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(m + k + n)
+    x, w = _grid(m, k, gen), _grid(n, k, gen)
+    q = ops.mx_quantize(w)
+    for out in {torch.float32, TYPES[name]}:
+        _assert_exact(ops.mx_linear(x.to(TYPES[name]), *q, None, n, k, out_dtype=out), x, w.t(), 1 / 16, (_mx_forms.product_form(m, k, n), out))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("m,k,n", _mx_forms.GRADIENTS)
+def test_gradients_of_every_form_are_exact(cuda_device, m, k, n, name):
+    """dy has as many bits as the sums leave room for: more than one bf16 term of fp16 and fp32 where they are short."""
+    from dimq_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(m + k + n)
+    dtype = TYPES[name]
+    w, x8, x4 = _grid(n, k, gen), _bytes(m, k, gen), _grid(m, k, gen)
+
+    def grad(depth, unit):       # values up to 2 in steps of 2^-bits, with room for `depth` products of them
+        bits = max(0, min(6 if name == "bf16" else 8, int(math.log2(2.0 ** 24 * unit / (8.0 * depth)))))
+        return (torch.randint(-2 << bits, (2 << bits) + 1, (m, n), device="cuda", generator=gen) / 2.0 ** bits).to(dtype), 2.0 ** -bits * unit
+
+    for out in {torch.float32, dtype}:
+        dy, unit = grad(n, 1 / 4)
+        _assert_exact(ops.mx_linear_grad_input(dy, *ops.mx_quantize(w), k, out_dtype=out), dy, w, unit,
+                      ("dx", _mx_forms.gradient_form(m, k, n, _mx_forms.TERMS[name])))
+        for fmt, x, step in (("int8", x8, 1 / 128), ("fp4", x4, 1 / 4)):
+            dy, unit = grad(m, step)
+            _assert_exact(ops.mx_linear_grad_weight(dy, *ops.mx_quantize(x, fmt), k, fmt, out_dtype=out), dy.t(), x, unit,
+                          ("dw " + fmt, _mx_forms.gradient_form(n, k, m, _mx_forms.TERMS[name])))
+
+
+@pytest.mark.parametrize("m,k,n", _mx_forms.GRADIENTS)
+def test_all_bits_of_an_fp32_gradient_count(cuda_device, m, k, n):
+    """Twenty bits of dy, in few places: the three terms of every one of them are in the sums."""
+    from dimq_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(m + k + n + 1)
+    w, x8 = _grid(n, k, gen), _bytes(m, k, gen)
+    far = torch.randint(-2 ** 20, 2 ** 20 + 1, (m, n), device="cuda", generator=gen).float()
+    row = torch.arange(m, device="cuda")
+    dy = torch.zeros(m, n, device="cuda")
+    col = torch.randint(0, n, (m,), device="cuda", generator=gen)
+    dy[row, col] = far[row, col] / 2.0 ** 10            # one value a row: dx is a multiple of a row of w
+    dx = ops.mx_linear_grad_input(dy, *ops.mx_quantize(w), k).double()
+    want = dy.double() @ w.double()
+    # three exact products added up, largest last: two roundings or cuts
+    assert float(((dx - want).abs() - 2.0 ** -22 * want.abs()).max()) <= 0
+    dy = torch.zeros(m, n, device="cuda")
+    other = torch.randint(0, m, (n,), device="cuda", generator=gen)
+    at = torch.arange(n, device="cuda")
+    dy[other, at] = far[other, at] / 2.0 ** 10          # one value a column: dw is a multiple of a row of x
+    dw = ops.mx_linear_grad_weight(dy, *ops.mx_quantize(x8, "int8"), k).double()
+    want = dy.double().t() @ x8.double()
+    assert float(((dw - want).abs() - 2.0 ** -22 * want.abs()).max()) <= 0
