@@ -5,8 +5,11 @@
 // brings codes (rows of 128 bytes = 256 values, 128-byte swizzle) and the 512-byte scale tiles that the format keeps,
 // tcgen05.cp moves a scale tile to tensor memory, and the accumulators go through bias, activation and residual to y.
 // Products are multiples of a quarter of their blocks' scales and 64 of them take one step, so the cut to fp32 at each step
-// rarely loses a bit: against 64 bits the sums of normal values are exact (K = 32768), those of blocks whose scales differ by
-// 2^12 and more are within 1.2e-7 (K = 11008) to 6.9e-7 (K = 32768).
+// often loses nothing: the sums of normal values, of mixed or one sign, are exact (K = 32768).  Where scales are spread, each
+// step cuts up to 2^-23 of the sum, always towards zero (relative Frobenius norms at K = 8192 / 32768): scales over 2^+-4 on
+// either side, mixed signs, 1.3e-7 / 7.9e-7; over 2^+-12, 2.6e-6 / 1.0e-5; over 2^+-6, all of one sign, 1.7e-6 / 8.0e-6.  An
+// fp32 torch.matmul of the same values is off by 1.4e-7 / 4.5e-7, 6.3e-7 / 1.2e-6 and 5.5e-6 / 2.9e-5 (1300 x 2600).  Adding up
+// parts of K in registers would bring these down; it took 58 us instead of 40 (2048 x 11008 -> 2048) and was left out.
 //
 // Large problems run on pairs of blocks (cta_group::2): 256 x 256 tiles, each block holding its 128 rows of x and half of
 // the tile's rows of w, so that a step moves 32 KB of codes into each shared memory instead of 48.  The first block of a

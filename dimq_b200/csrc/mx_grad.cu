@@ -7,7 +7,8 @@
 // in panels of 64 columns, so that one copy brings all of a tile's), and the operand descriptors say that the columns are contiguous ("MN major") - w^ and x~ always, dy for dw.
 //
 // dy enters exactly: bf16 as it is, fp16 and fp32 as the sum of two or three bf16 terms, each the leading eight bits of
-// what the ones before left (24 bits in all; an infinity or a NaN is its own first term).  The terms are passes over the
+// what the ones before left (24 bits in all; an infinity or a NaN is its own first term).  bf16 has no bits under 2^-133, so an
+// fp32 value loses what it has there: nothing above 2^-110, under 2.5e-7 of one of 2^-112, 6e-5 of 2^-120, 4e-3 of 2^-126.  The terms are passes over the
 // same reduction, smallest first.
 //
 // The tensor cores cut their sums to fp32 instead of rounding them: the error grows with the number of steps.  Where the

@@ -382,9 +382,10 @@ DIMQ_API int dimq_mx_linear(const void* x, int x_dtype, const uint8_t* x_scales,
                             int64_t K, int epilogue, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Gradients of that layer, straight through the quantisation: dx [M][K] = dy w^ and dw [N][K] = dy^T x~, db [N] the column
- * sums of dy [M][N] (dw or db may be NULL; without dw nothing of x is read).  x~ is what x_codes / x_scales hold (either format: the 8-bit copy is what a layer
- * keeps of its activations).  dy (16-byte aligned) is taken exactly, sums in fp32.  Scratch for either: dimq_mx_grad_workspace_bytes,
- * 256-byte aligned. */
+ * sums of dy [M][N] (dw or db may be NULL; without dw nothing of x is read).  x~ is what x_codes / x_scales hold (either
+ * format: the 8-bit copy is what a layer keeps of its activations).  dy (16-byte aligned) is taken exactly, but that the
+ * products drop an fp32 dy's bits under 2^-133; sums in fp32.  Scratch for either: dimq_mx_grad_workspace_bytes, 256-byte
+ * aligned. */
 DIMQ_API int dimq_mx_grad_workspace_bytes(int dy_dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes);
 DIMQ_API int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, void* dx,
                                 int dx_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,

@@ -124,3 +124,99 @@ def test_all_bits_of_an_fp32_gradient_count(cuda_device, m, k, n):
     dw = ops.mx_linear_grad_weight(dy, *ops.mx_quantize(x8, "int8"), k).double()
     want = dy.double().t() @ x8.double()
     assert float(((dw - want).abs() - 2.0 ** -22 * want.abs()).max()) <= 0
+
+
+# ---- sums that fp32 has to round -------------------------------------------------------------------
+
+LONG = [(8, 32768, 256), (64, 32768, 256), (200, 11008, 8200), (300, 11008, 10200), (1300, 11008, 2600)]     # one of each form
+
+
+def _values_of(x, fmt="fp4"):
+    from dimq_b200 import ops
+
+    codes, scales = ops.mx_quantize(x, fmt)
+    return ops.mx_dequantize(codes, scales, x.shape[1], fmt).double(), int(ops.mx_scale_rows(scales, *x.shape).min()) - 127
+
+
+@pytest.mark.parametrize("m,k,n", LONG)
+def test_long_sums_of_normal_values_are_exact(cuda_device, m, k, n):
+    """Normal values, mixed and of one sign: the codes have so few bits that no sum of 32768 products needs more than 24."""
+    from dimq_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for sign in (False, True):
+        x, w = torch.randn(m, k, device="cuda", generator=gen), 0.02 * torch.randn(n, k, device="cuda", generator=gen)
+        if sign:
+            x, w = x.abs(), w.abs()
+        (a, low_a), (b, low_b) = _values_of(x), _values_of(w)
+        _assert_exact(ops.mx_linear(x, *ops.mx_quantize(w), None, n, k), a, b.t(), 2.0 ** (low_a + low_b - 2), sign)
+
+
+@pytest.mark.parametrize("spread", [4, 12])
+@pytest.mark.parametrize("m,k,n", LONG)
+def test_long_sums_of_spread_blocks(cuda_device, m, k, n, spread):
+    """Blocks up to 2^(4 spread) apart in their products, of mixed and of one sign.
+
+    Bound: 64 products take one step of the tensor cores, each cutting the sum by at most a step of 2^-23 of it, a sum is at
+    most sum |a||b|, and up to eight parts are added in fp32.  That is K / 64 + 9 cuts, where a bound over all K additions would
+    let a 64-k step go missing."""
+    from dimq_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(2)
+
+    def values(rows):
+        e = torch.randint(-spread, spread + 1, (rows, k // 32), device="cuda", generator=gen).float()
+        return torch.randn(rows, k, device="cuda", generator=gen) * torch.exp2(e).repeat_interleave(32, 1)
+
+    for sign in (False, True):
+        x, w = values(m), values(n)
+        if sign:
+            x, w = x.abs(), w.abs()
+        a, b = _values_of(x)[0], _values_of(w)[0].t()
+        y = ops.mx_linear(x, *ops.mx_quantize(w), None, n, k).double()
+        bound = (k / 64 + 9) * 2.0 ** -23 * (a.abs() @ b.abs())
+        assert float(((y - a @ b).abs() - bound).max()) <= 0, sign
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("m,k,n", [(9000, 200, 264), (40, 136, 5000), (20000, 72, 264), (700, 2600, 1300)])
+def test_long_gradient_sums_of_spread_values(cuda_device, m, k, n, name):
+    """As above for the gradients: 16 products a step of the tensor cores, each off by at most two units of 2^-23 of a sum that
+    is at most sum |a||b|; fp32 results are added up every 512 values of each term (32 steps, and one addition for every 512)."""
+    from dimq_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x, w = torch.randn(m, k, device="cuda", generator=gen), torch.randn(n, k, device="cuda", generator=gen)
+    x *= torch.exp2(3 * torch.randn(m, 1, device="cuda", generator=gen))       # scales along the reduction
+    w *= torch.exp2(3 * torch.randn(n, 1, device="cuda", generator=gen))
+    dy = torch.randn(m, n, device="cuda", generator=gen).to(TYPES[name])
+    terms = _mx_forms.TERMS[name]
+    for out in {torch.float32, TYPES[name]}:
+        for got, a, b, depth in ((ops.mx_linear_grad_input(dy, *ops.mx_quantize(w), k, out_dtype=out), dy, _values_of(w)[0], n),
+                                 (ops.mx_linear_grad_weight(dy, *ops.mx_quantize(x, "int8"), k, out_dtype=out), dy.t(), _values_of(x, "int8")[0], m)):
+            a = a.double()
+            steps = 32 + terms * depth / 512 + 18 if out == torch.float32 else terms * depth / 16 + 34
+            want = a @ b
+            bound = 2 * steps * 2.0 ** -23 * (a.abs() @ b.abs())
+            if out != torch.float32:
+                bound = bound + torch.finfo(out).eps / 2 * (want.abs() + bound)
+            assert float(((got.double() - want).abs() - bound).max()) <= 0, (out, depth)
+
+
+def test_small_fp32_gradients(cuda_device):
+    """An fp32 gradient enters as three bf16 terms, and bf16 has no bits under 2^-133: a value loses less than that, nothing else."""
+    from dimq_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    m, k, n = 70, 64, 96
+    w, x = torch.randn(n, k, device="cuda", generator=gen) * 2.0 ** 60, torch.randn(m, k, device="cuda", generator=gen) * 2.0 ** 60
+    for power in (-108, -112, -120, -126, -130):
+        dy = torch.randn(m, n, device="cuda", generator=gen) * 2.0 ** power
+        for got, a, b, depth in ((ops.mx_linear_grad_input(dy, *ops.mx_quantize(w), k), dy, _values_of(w)[0], n),
+                                 (ops.mx_linear_grad_weight(dy, *ops.mx_quantize(x, "int8"), k), dy.t(), _values_of(x, "int8")[0], m)):
+            a = a.double()
+            lost = 2.0 ** -133 * b.abs().sum(0)
+            bound = lost + 2 * (3 * depth / 16 + 20) * 2.0 ** -23 * (a.abs() @ b.abs())
+            assert float(((got.double() - a @ b).abs() - bound).max()) <= 0, power
+            if power == -108:        # what is lost is under a quarter of a step of 2^-23 of a value of this size
+                assert float((lost / (2.0 ** power * b.abs().sum(0))).max()) <= 2.0 ** -25
