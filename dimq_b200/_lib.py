@@ -33,7 +33,7 @@ EXPORTED_SYMBOLS = (
     "dimq_linear_wq_workspace_bytes", "dimq_linear_wq_ws", "dimq_linear_wq_ws_plan", "dimq_expand_workspace_bytes", "dimq_linear_wq_expand",
     "dimq_linear_wq_regs_workspace_bytes", "dimq_linear_wq_regs", "dimq_linear_prepack",
     "dimq_conv2d_wq_workspace_bytes", "dimq_conv2d_wq_ws", "dimq_conv2d_wq_expand", "dimq_selftest_bounded_wait", "dimq_mx_sizes", "dimq_mx_quantize", "dimq_mx_quantize_both", "dimq_mx_dequantize",
-    "dimq_mx_linear_workspace_bytes", "dimq_mx_linear", "dimq_mx_grad_workspace_bytes", "dimq_mx_grad_input",
+    "dimq_mx_linear_workspace_bytes", "dimq_mx_linear", "dimq_mx_grad_workspace_bytes", "dimq_mx_grad_launches", "dimq_mx_grad_input",
     "dimq_mx_grad_weight", "dimq_mx_grads", "dimq_fake_quantize_ste", "dimq_centre_quantize_u4",
 )
 

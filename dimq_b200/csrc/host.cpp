@@ -930,6 +930,12 @@ Tensor once_of(const Tensor& grad, Tensor result, const char* what) {
   return one[0];
 }
 
+int mx_grad_launches(int dyd, int64_t m, int64_t n, int64_t k, bool dx, bool dw, bool db) {
+  int kernels = 0;
+  check(dimq_mx_grad_launches(dyd, m, n, k, dx, dw, db, &kernels), "mx_grad_launches");
+  return kernels;
+}
+
 Tensor mx_grad_scratch(const Tensor& dy, int dyd, int64_t m, int64_t n, int64_t k, int64_t* need) {
   check(dimq_mx_grad_workspace_bytes(dyd, m, n, k, need), "mx_grad_workspace_bytes");
   return scratch(*need, dy);
@@ -951,7 +957,7 @@ Tensor mx_grad_input(const Tensor& dy, const Tensor& codes, const Tensor& scales
   const Tensor ws = mx_grad_scratch(g, dyd, m, n, k, &need);
   check(dimq_mx_grad_input(g.data_ptr(), dyd, bytes_of(w.codes), bytes_of(w.scales), dx.data_ptr(), dtype_code(dx, "out_dtype"), m, n,
                            k, ws.data_ptr(), need, stream_of(dy)), "mx_linear_grad_input");
-  *launches += m > 0 ? 2 : 0;
+  *launches += mx_grad_launches(dyd, m, n, k, true, false, false);
   return dx;
 }
 
@@ -971,7 +977,7 @@ Tensor mx_grad_weight(const Tensor& dy, const Tensor& codes, const Tensor& scale
   const Tensor ws = mx_grad_scratch(g, dyd, m, n, k, &need);
   check(dimq_mx_grad_weight(g.data_ptr(), dyd, x.codes.data_ptr(), bytes_of(x.scales), format, dw.data_ptr(), dtype_code(dw, "out_dtype"),
                             nullptr, 0, m, n, k, ws.data_ptr(), need, stream_of(dy)), "mx_linear_grad_weight");
-  *launches += m > 0 ? 2 : 0;
+  *launches += mx_grad_launches(dyd, m, n, k, false, true, false);
   return dw;
 }
 
@@ -1042,7 +1048,7 @@ class MxProduct : public torch::autograd::Function<MxProduct> {
                             need_x ? dx.data_ptr() : nullptr, need_x ? dtype_code(dx, "gradient") : 0, nullptr, 0,
                             need_b ? db.data_ptr() : nullptr, need_b ? dtype_code(db, "gradient") : 0, m, n, k, ws.data_ptr(), need,
                             stream_of(g)), "mx_grads");
-        launches += m > 0 ? 2 * need_x + need_b : 0;
+        launches += mx_grad_launches(dzd, m, n, k, need_x, false, need_b);
         out[0] = dx;
         out[3] = db;
       }
@@ -1124,7 +1130,7 @@ class MxLayer : public torch::autograd::Function<MxLayer> {
       check(dimq_mx_grads(g.data_ptr(), dyd, need_x ? w.codes() : nullptr, need_x ? w.scales() : nullptr, need_w ? x.codes() : nullptr,
                           need_w ? x.scales() : nullptr, keep, at_or_null(dx), dtype_of(dx), at_or_null(dw), dtype_of(dw), at_or_null(db),
                           dtype_of(db), m, n, k, ws.data_ptr(), need, stream_of(g)), "mx_grads");
-    count_launches_no_gil(m > 0 ? 2 * need_x + 2 * need_w + need_b : 0);
+    count_launches_no_gil(mx_grad_launches(dyd, m, n, k, need_x, need_w, need_b));
     out[0] = dx;
     out[1] = dw;
     out[2] = db;

@@ -571,6 +571,20 @@ extern "C" int dimq_mx_grad_workspace_bytes(int dy_dtype, int64_t M, int64_t N, 
   return DIMQ_OK;
 }
 
+extern "C" int dimq_mx_grad_launches(int dy_dtype, int64_t M, int64_t N, int64_t K, int dx, int dw, int db, int* kernels) {
+  if (kernels == nullptr) return DIMQ_ERR_NULL_POINTER;
+  *kernels = 0;
+  if (!valid_dtype(dy_dtype)) return DIMQ_ERR_BAD_DTYPE;
+  const int rc = check_sizes(M, N, K);
+  if (rc != DIMQ_OK || M == 0) return rc;
+  const int terms = terms_of(dy_dtype);
+  if (db) *kernels += 1 + (M > kSumRows);                                             // runs, their sum
+  if ((dx || dw) && !as_it_is(dy_dtype, N)) *kernels += 1;                            // terms
+  if (dx) *kernels += 2 + (plan_of(M, K, N, terms).slices > 1);                       // decode, product, sum of slices
+  if (dw) *kernels += 2 + (plan_of(N, K, M, terms).slices > 1);
+  return DIMQ_OK;
+}
+
 // dx (null: not wanted) from w, dw (null) from x, db (null); dy's terms are made once
 static int grads(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, const void* x_codes,
                  const uint8_t* x_scales, int format, void* dx, int dx_dtype, void* dw, int dw_dtype, void* db, int db_dtype, int64_t M,

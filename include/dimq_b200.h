@@ -387,6 +387,8 @@ DIMQ_API int dimq_mx_linear(const void* x, int x_dtype, const uint8_t* x_scales,
  * products drop an fp32 dy's bits under 2^-133; sums in fp32.  Scratch for either: dimq_mx_grad_workspace_bytes, 256-byte
  * aligned. */
 DIMQ_API int dimq_mx_grad_workspace_bytes(int dy_dtype, int64_t M, int64_t N, int64_t K, int64_t* bytes);
+/* Kernels that the call computing these (dx, dw, db: whether wanted) launches. */
+DIMQ_API int dimq_mx_grad_launches(int dy_dtype, int64_t M, int64_t N, int64_t K, int dx, int dw, int db, int* kernels);
 DIMQ_API int dimq_mx_grad_input(const void* dy, int dy_dtype, const uint8_t* w_codes, const uint8_t* w_scales, void* dx,
                                 int dx_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                                 void* stream);
