@@ -220,9 +220,8 @@ __device__ __forceinline__ float gelu_wide(float v) { return 0.5f * v * erfcf(v 
 
 // RELU, ADD_RELU or none
 __device__ __forceinline__ float activate_linear(float v, float res, int epilogue) {
-  if (epilogue == DIMQ_EPI_ADD_RELU) return max_nan(v + res, 0.0f);
-  if (epilogue == DIMQ_EPI_RELU) v = max_nan(v, 0.0f);
-  return v + res;
+  if (epilogue == DIMQ_EPI_NONE) return v + res;
+  return epilogue == DIMQ_EPI_ADD_RELU ? max_nan(v + res, 0.0f) : max_nan(v, 0.0f) + res;
 }
 template <bool WIDE>
 __device__ __forceinline__ float activate_any(float v, float res, int epilogue) {
@@ -257,8 +256,9 @@ constexpr uint32_t kStagingBytes = 4096;
 // sums change hands through shared memory, so that a warp stores 32 neighbours of one row at a time.  (Boxes of 64 columns,
 // and 16-byte stores of four rows at a time instead of the map, were slower: 25216 x 768 -> 2304 bf16 59 and 69 us against
 // 57.)
-// GELU of fp32 is done in the box, four values at a time: unrolled over the row in registers it would not fit.  (ACT: whether
-// there can be an activation.)
+// GELU of fp32 is done in the box, four values at a time: unrolled over the row in registers it would not fit.  It costs the
+// instructions of erfc: 2048 x 1024 -> 4096 35.6 us (the polynomial 28.9, ReLU 15.0; 8 and 16 values at a time 37 and 39).
+// (ACT: whether there can be an activation.)
 template <int ES, bool ACT = true>
 __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CUtensorMap* map, unsigned char* stage, uint32_t& turn,
                                           const float* bias, int64_t row0, int64_t n0, int lane) {
@@ -352,11 +352,21 @@ __device__ __forceinline__ void put_chunk(float (&v)[32], const Out& o, const CU
   const float b = bias != nullptr ? bias[lane] : 0.0f;
   if (n < o.cols) {
     const int rows = static_cast<int>(o.rows - row0 < 32 ? o.rows - row0 : 32);
+    if (ES == 4 && ACT && o.epilogue == DIMQ_EPI_GELU) {   // apart: it is long
 #pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-      const int64_t at = (row0 + r) * o.cols + n;
-      const float res = o.residual != nullptr ? load_as_float(o.residual, o.dtype, at) : 0.0f;
-      store_from_float(o.y, o.dtype, at, ACT ? activate_any<ES == 4>(f[r * 32 + (lane ^ r)] + b, res, o.epilogue) : f[r * 32 + (lane ^ r)] + b);
+      for (int r = 0; r < rows; ++r) {
+        const int64_t at = (row0 + r) * o.cols + n;
+        const float res = o.residual != nullptr ? static_cast<const float*>(o.residual)[at] : 0.0f;
+        static_cast<float*>(o.y)[at] = gelu_wide(f[r * 32 + (lane ^ r)] + b) + res;
+      }
+    } else {
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r) {
+        const int64_t at = (row0 + r) * o.cols + n;
+        const float res = o.residual != nullptr ? load_as_float(o.residual, o.dtype, at) : 0.0f;
+        const float v = f[r * 32 + (lane ^ r)] + b;
+        store_from_float(o.y, o.dtype, at, ES == 2 && ACT ? activate_any<false>(v, res, o.epilogue) : activate_linear(v, res, o.epilogue));
+      }
     }
   }
   __syncwarp();
