@@ -1062,11 +1062,16 @@ class MxProduct : public torch::autograd::Function<MxProduct> {
   }
 };
 
+// Whether a gradient has to come back for t, or t carries a forward-mode tangent (which the nodes here refuse)
+bool differentiated(const Tensor& t) {
+  return t.unsafeGetTensorImpl()->autograd_meta() != nullptr &&     // plain tensors have none
+         ((t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined());
+}
+
 // The product of the Python entry point: an autograd node where a gradient has to come back.
 Tensor mx_product(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& bias, int64_t n, int64_t k,
                   at::ScalarType out_dtype, int epilogue, const OptTensor& residual, int* launches) {
-  if (at::GradMode::is_enabled() &&
-      (x.requires_grad() || (bias.has_value() && bias->requires_grad()) || (residual.has_value() && residual->requires_grad())))
+  if (differentiated(x) || (bias.has_value() && differentiated(*bias)) || (residual.has_value() && differentiated(*residual)))
     return MxProduct::apply(x, codes, scales, bias, residual, n, k, static_cast<int64_t>(out_dtype), static_cast<int64_t>(epilogue));
   return mx_linear(x, codes, scales, bias, n, k, out_dtype, epilogue, residual, launches);
 }

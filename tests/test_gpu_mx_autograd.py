@@ -157,3 +157,22 @@ def test_frozen_layer_inside_a_trained_model(cuda_device):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, eager)
+
+
+def test_forward_mode_tangents_are_refused(cuda_device):
+    """There is no forward-mode rule: a tangent raises instead of getting lost."""
+    from torch.autograd import forward_ad
+
+    from dimq_b200 import ops, qat
+
+    m, k, n = 20, 64, 24
+    w = _on_grid(n, k, 9).cuda()
+    q = ops.mx_quantize(w)
+    x, b, r = _on_grid(m, k, 10).cuda(), torch.randn(n, device="cuda"), torch.randn(m, n, device="cuda")
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, b, r)]
+        for call in (lambda: ops.mx_linear(dual[0], *q, b, n, k), lambda: ops.mx_linear(x, *q, dual[1], n, k),
+                     lambda: ops.mx_linear(x, *q, b, n, k, residual=dual[2]), lambda: qat.mx_linear(dual[0], w)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+        assert not ops.mx_linear(x, *q, b, n, k).requires_grad
